@@ -36,6 +36,7 @@ extern "C" {
 #define MK_TYPE_Q8_0 8
 #define MK_TYPE_Q4_K 12
 #define MK_TYPE_Q6_K 14
+#define MK_TYPE_BF16 30
 
 #define MK_MAX_DRAFT 32 /* draft tokens per request per step (malkin: n_draft <= kMaxBatch - 1, adaptive <= 8) */
 
@@ -328,6 +329,61 @@ int mk_attention(const float* dev_q, int n, int H, int KV, int D, const int8_t* 
                  const float* dev_ks, const float* dev_vs, int64_t n_rows, const int32_t* dev_kv_base,
                  const int32_t* dev_n_keys, const int32_t* dev_anc_off, const int32_t* dev_anc, float* dev_out,
                  void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Serving operators for callers that keep their own model, on the current device, on device buffers. They stand beside
+ * the kernel-level entry points above with two differences: they take 16-bit activations and use the tensor cores, so
+ * their sums are not in malkin's operation order (results agree with it to the rounding of the types); and they only
+ * queue work on `stream`: no allocation, no synchronization, so they can be captured into a CUDA graph.
+ *
+ * Index tables are device memory and can change between replays. The kernels check every index they follow; what is out
+ * of range is skipped as each call says and, when dev_status is not NULL, recorded there: the caller clears
+ * the word, the first code found (MK_ERR_ARG, MK_ERR_TIMEOUT) is stored into it. Shapes, strides, alignment and the
+ * device of every pointer are checked by the call itself (MK_ERR_ARG). Strides (ld) are in elements of the buffer.
+ * Input and output buffers must not overlap unless a call says so. A workspace belongs to one call until the
+ * stream has passed it: calls that may run at the same time, and graphs that may, need one each.
+ * ------------------------------------------------------------------------------------------------------- */
+
+/* RMSNorm of each query and key head and the position rotation in one pass (Model::run's q / k norm and rope,
+ * model.cpp:336-360), with the int8 cache rows of the same tokens. type: MK_TYPE_F32, MK_TYPE_F16 or MK_TYPE_BF16.
+ * dev_qkv: n rows of H query heads, KV key heads, KV value heads of D values each (D 64, 128 or 256), ld apart;
+ * dev_q_norm / dev_k_norm: D float weights; dev_rope: n_pos rows [cos D/2 | sin D/2] of floats, pairs (i, i + D/2);
+ * dev_pos: n rows of that table. dev_q: n rows of H x D, q_ld apart; dev_k: n rows of KV x D, k_ld apart (NULL: none).
+ * In place is allowed: dev_q = dev_qkv with q_ld = ld, dev_k = its key heads with k_ld = ld.
+ * dev_kc / dev_vc (NULL: no cache): int8 [KV][n_rows][D] with float row scales dev_ks / dev_vs [KV][n_rows]; the rotated
+ * key head and the value head of token t are quantized (quantize_i8, quant.cpp:134-140) from their fp32 values into row
+ * dev_kv_at[t]. Two tokens with the same row leave either's values there.
+ * A token with dev_pos[t] < 0 is padding: nothing of it is written; dev_kv_at[t] < 0: no cache row of it is written.
+ * dev_pos[t] >= n_pos or dev_kv_at[t] >= n_rows does the same and records MK_ERR_ARG. */
+int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int KV, int D, const float* dev_q_norm,
+                    const float* dev_k_norm, float eps, const float* dev_rope, int n_pos, const int32_t* dev_pos,
+                    void* dev_q, int64_t q_ld, void* dev_k, int64_t k_ld, int8_t* dev_kc, int8_t* dev_vc, float* dev_ks,
+                    float* dev_vs, int64_t n_rows, const int32_t* dev_kv_at, int32_t* dev_status, void* stream);
+
+/* Verification of drafted tokens over the whole vocabulary: Engine::accept_sampled / accept_greedy's chain and
+ * Sampler::verify / draw (engine.cpp:441-507, sampler.cpp:64-97) with softmax(logits / temperature) of all V tokens
+ * where mk_accept works on at most MK_MAX_TOPK candidates (no top-k, top-p or min-p here).
+ * Request r has logits rows dev_row_off[r] .. dev_row_off[r + 1] - 1 (at least one; dev_row_off has n_req + 1 ascending
+ * entries, the last at most n_rows): k = their count - 1 drafted tokens, draft i verified by row dev_row_off[r] + i.
+ * Drafts are packed: that of row x of request r is dev_draft[x - r], its probabilities row x - r of dev_q (V floats,
+ * q_ld apart). dev_q NULL: every draft counts as certain (probability 1). dev_logits: n_rows rows of V values of `type`
+ * (MK_TYPE_F32, MK_TYPE_F16, MK_TYPE_BF16), ld apart. dev_uniforms: n_rows doubles in [0, 1); request r uses those at
+ * dev_row_off[r] .. in the sampler's order: one per draft looked at, then one for the draw.
+ * temperature > 0: draft d is kept while q(d) > 0 and u q(d) < p(d); at the first that is not, the next token is drawn
+ * from max(p - q, 0) (from p where that is 0 everywhere), after the last from p of the last row: the lowest token whose
+ * running sum in index order reaches u x the total. temperature <= 0 (or NaN): kept while it is the row's argmax (the
+ * lowest index of the maximum), next = argmax; dev_q and the uniforms are not used.
+ * Results: dev_n_acc[r] drafts kept, dev_next[r], dev_p[x - r] (NULL: not wanted) the target's probability of each draft
+ * looked at, 0 for those after the first one that was not kept. A draft outside 0 .. V - 1 has probability 0. Logits of
+ * -infinity are tokens that cannot be drawn, NaN logits count as -infinity; a row whose maximum is not finite has no
+ * distribution: no draft is kept on it, and as the row drawn from it gives dev_next = -1. A request whose rows are not as
+ * above gives dev_n_acc = 0, dev_next = -1 and records MK_ERR_ARG (its dev_p entries are not written).
+ * dev_ws: mk_verify_draft_workspace(n_rows, n_req, V) bytes, 16-byte aligned. V at most 2^27. */
+int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V);
+int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,
+                    const int32_t* dev_row_off, const int32_t* dev_draft, const float* dev_q, int64_t q_ld,
+                    const float* dev_temperature, const double* dev_uniforms, int32_t* dev_n_acc, int32_t* dev_next,
+                    float* dev_p, void* dev_ws, int64_t ws_bytes, int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

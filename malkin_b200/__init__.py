@@ -205,7 +205,8 @@ EXPORTS = ("mk_last_error", "mk_version", "mk_synth_gguf", "mk_init", "mk_nccl_u
            "mk_stream", "mk_last_io_bytes", "mk_tp_shard_of", "mk_tp_exchange_check", "mk_weight_upload", "mk_weight_free", "mk_weight_device_bytes", "mk_quantize_q8",
            "mk_matmul", "mk_matmul_noalloc", "mk_block_dots", "mk_quantize_i8", "mk_silu_mul", "mk_attention",
            "mk_engine_create", "mk_engine_destroy", "mk_engine_submit", "mk_engine_step", "mk_engine_events",
-           "mk_engine_busy", "mk_engine_cancel", "mk_engine_stats", "mk_engine_perplexity")
+           "mk_engine_busy", "mk_engine_cancel", "mk_engine_stats", "mk_engine_perplexity", "mk_qk_norm_rope",
+           "mk_verify_draft_workspace", "mk_verify_draft")
 
 
 def version() -> str:
@@ -502,3 +503,41 @@ def attention(dev_q: int, n: int, H: int, KV: int, D: int, dev_k: int, dev_v: in
               stream: int = 0) -> None:
     _check(lib.mk_attention(dev_q, n, H, KV, D, dev_k, dev_v, dev_ks, dev_vs, n_rows, dev_kv_base, dev_n_keys,
                             dev_anc_off, dev_anc, dev_out, stream or None))
+
+
+# ---- serving operators (device pointers; they queue work on `stream` and return) ----
+lib.mk_qk_norm_rope.argtypes = [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                ctypes.c_int, _vp, _vp, ctypes.c_float, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int64,
+                                _vp, ctypes.c_int64, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, _vp, _vp]
+lib.mk_verify_draft_workspace.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int]
+lib.mk_verify_draft_workspace.restype = ctypes.c_int64
+lib.mk_verify_draft.argtypes = [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp,
+                                _vp, ctypes.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, _vp]
+
+
+def qk_norm_rope(type_: int, dev_qkv: int, ld: int, n: int, H: int, KV: int, D: int, dev_q_norm: int, dev_k_norm: int,
+                 eps: float, dev_rope: int, n_pos: int, dev_pos: int, dev_q: int, q_ld: int, dev_k: int = 0,
+                 k_ld: int = 0, dev_kc: int = 0, dev_vc: int = 0, dev_ks: int = 0, dev_vs: int = 0, n_rows: int = 0,
+                 dev_kv_at: int = 0, dev_status: int = 0, stream: int = 0) -> None:
+    """q / k norm per head and rotation in one pass, with the int8 cache rows of the same tokens (mk_qk_norm_rope).
+    type_: TYPE_F32, TYPE_F16 or TYPE_BF16; strides in elements."""
+    _check(lib.mk_qk_norm_rope(type_, dev_qkv, ld, n, H, KV, D, dev_q_norm, dev_k_norm, eps, dev_rope, n_pos, dev_pos,
+                               dev_q, q_ld, dev_k or None, k_ld, dev_kc or None, dev_vc or None, dev_ks or None,
+                               dev_vs or None, n_rows, dev_kv_at or None, dev_status or None, stream or None))
+
+
+def verify_draft_workspace(n_rows: int, n_req: int, V: int) -> int:
+    """Workspace bytes of verify_draft."""
+    b = lib.mk_verify_draft_workspace(n_rows, n_req, V)
+    if b < 0:
+        raise MalkinError(MK_ERR_ARG, "verify_draft_workspace: bad shape")
+    return b
+
+
+def verify_draft(type_: int, dev_logits: int, ld: int, n_rows: int, V: int, n_req: int, dev_row_off: int,
+                 dev_draft: int, dev_q: int, q_ld: int, dev_temperature: int, dev_uniforms: int, dev_n_acc: int,
+                 dev_next: int, dev_p: int, dev_ws: int, ws_bytes: int, dev_status: int = 0, stream: int = 0) -> None:
+    """Verification of drafted tokens over the whole vocabulary (mk_verify_draft)."""
+    _check(lib.mk_verify_draft(type_, dev_logits, ld, n_rows, V, n_req, dev_row_off, dev_draft or None, dev_q or None,
+                               q_ld, dev_temperature, dev_uniforms, dev_n_acc, dev_next, dev_p or None, dev_ws,
+                               ws_bytes, dev_status or None, stream or None))

@@ -3,6 +3,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <random>
 #include <stdexcept>
@@ -84,6 +85,56 @@ int current_device() {
   int d = 0;
   mkb::cuda_check(cudaGetDevice(&d), "cudaGetDevice");
   return d;
+}
+
+// ---- checks of the serving operators ----
+constexpr int kMaxHeads = 1024;
+constexpr int kMaxVocab = 1 << 27;
+constexpr int kMaxReq = 1 << 20;
+
+mkb::ActType act_type(int type, bool with_f32, const char* who) {
+  if (type == MK_TYPE_F32 && with_f32) return mkb::ActType::f32;
+  if (type == MK_TYPE_F16) return mkb::ActType::f16;
+  if (type == MK_TYPE_BF16) return mkb::ActType::bf16;
+  throw mkb::ArgError(std::string(who) + ": type must be " + (with_f32 ? "F32, F16 or BF16" : "F16 or BF16"));
+}
+size_t act_size(mkb::ActType t) { return t == mkb::ActType::f32 ? 4 : 2; }
+
+struct DevArg {
+  const void* p;
+  size_t align;
+  const char* name;
+  bool optional = false;
+};
+// Every pointer is device memory of the current device, on its alignment: a host pointer or another GPU's is refused
+// here, where it would fault in the kernel.
+void check_dev(std::initializer_list<DevArg> args, const char* who) {
+  for (const DevArg& a : args) {
+    if (!a.p && !a.optional) throw mkb::ArgError(std::string(who) + ": null " + a.name);
+    if (reinterpret_cast<uintptr_t>(a.p) % a.align)
+      throw mkb::ArgError(std::string(who) + ": " + a.name + " is not " + std::to_string(a.align) + "-byte aligned");
+  }
+  const int dev = current_device();
+  for (const DevArg& a : args) {
+    if (!a.p) continue;
+    cudaPointerAttributes at{};
+    mkb::cuda_check(cudaPointerGetAttributes(&at, a.p), who);
+    if (at.type == cudaMemoryTypeManaged) continue;
+    if (at.type != cudaMemoryTypeDevice)
+      throw mkb::ArgError(std::string(who) + ": " + a.name + " is not device memory");
+    if (at.device != dev)
+      throw mkb::ArgError(std::string(who) + ": " + a.name + " is on device " + std::to_string(at.device) +
+                          ", the current device is " + std::to_string(dev));
+  }
+}
+
+int current_sms() {
+  static int sms[mkb::kMaxDevices] = {};  // the same for every caller: a race writes the same value
+  const int dev = current_device();
+  if (dev >= mkb::kMaxDevices) throw mkb::UnsupportedError("device ordinal out of range");
+  if (!sms[dev])
+    mkb::cuda_check(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev), "device attribute");
+  return sms[dev];
 }
 
 // Temporary quantized-activation buffers for the kernel-level entry points: int8 qx | the same int8 values in the
@@ -505,6 +556,67 @@ int mk_attention(const float* dev_q, int n, int H, int KV, int D, const int8_t* 
     mkb::launch_attention(dev_q, H, KV, D, 1.0f / std::sqrt(static_cast<float>(D)), L, p, dev_out, mkb::ActQ{}, s);
     mkb::cuda_check(cudaGetLastError(), "attention");
     mkb::cuda_check(cudaStreamSynchronize(s), "attention");
+  });
+}
+
+// ---- serving operators ----
+
+int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int KV, int D, const float* dev_q_norm,
+                    const float* dev_k_norm, float eps, const float* dev_rope, int n_pos, const int32_t* dev_pos,
+                    void* dev_q, int64_t q_ld, void* dev_k, int64_t k_ld, int8_t* dev_kc, int8_t* dev_vc, float* dev_ks,
+                    float* dev_vs, int64_t n_rows, const int32_t* dev_kv_at, int32_t* dev_status, void* stream) {
+  return guard(MK_ERR_ARG, [&] {
+    const char* who = "qk_norm_rope";
+    const mkb::ActType t = act_type(type, true, who);
+    const bool cache = dev_kc || dev_vc || dev_ks || dev_vs;
+    const size_t size = act_size(t);
+    if (n < 0 || H <= 0 || KV <= 0 || H > kMaxHeads || KV > kMaxHeads || n_pos <= 0 || !std::isfinite(eps) || eps < 0.0f)
+      throw mkb::ArgError("qk_norm_rope: bad shape");
+    if (D != 64 && D != 128 && D != 256) throw mkb::ArgError("qk_norm_rope: head width must be 64, 128 or 256");
+    const int64_t width = static_cast<int64_t>(H + 2 * KV) * D;
+    if (ld < width || q_ld < static_cast<int64_t>(H) * D || (dev_k && k_ld < static_cast<int64_t>(KV) * D))
+      throw mkb::ArgError("qk_norm_rope: rows overlap (a stride is shorter than its row)");
+    if (cache && (n_rows <= 0 || !dev_kv_at)) throw mkb::ArgError("qk_norm_rope: a cache needs n_rows and dev_kv_at");
+    if (cache && (!dev_kc || !dev_vc || !dev_ks || !dev_vs))
+      throw mkb::ArgError("qk_norm_rope: the cache has four buffers, or none");
+    if (n == 0) return;
+    check_dev({{dev_qkv, size, "dev_qkv"}, {dev_q_norm, 4, "dev_q_norm"}, {dev_k_norm, 4, "dev_k_norm"},
+               {dev_rope, 4, "dev_rope"}, {dev_pos, 4, "dev_pos"}, {dev_q, size, "dev_q"}, {dev_k, size, "dev_k", true},
+               {dev_kc, 4, "dev_kc", true}, {dev_vc, 4, "dev_vc", true}, {dev_ks, 4, "dev_ks", true},
+               {dev_vs, 4, "dev_vs", true}, {cache ? dev_kv_at : nullptr, 4, "dev_kv_at", true},
+               {dev_status, 4, "dev_status", true}}, who);
+    mkb::NormRopeArgs a{dev_qkv, ld, n, H, KV, dev_q_norm, dev_k_norm, eps, dev_rope, n_pos, dev_pos, dev_q, q_ld,
+                        dev_k, k_ld, dev_kc, dev_vc, dev_ks, dev_vs, n_rows, dev_kv_at, dev_status};
+    mkb::launch_qk_norm_rope(a, t, D, current_sms(), as_stream(stream));
+    mkb::cuda_check(cudaGetLastError(), who);
+  });
+}
+
+int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V) {
+  if (n_rows < 0 || n_req < 0 || V <= 0 || V > kMaxVocab) return -1;
+  return mkb::verify_workspace(n_rows, V);
+}
+
+int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,
+                    const int32_t* dev_row_off, const int32_t* dev_draft, const float* dev_q, int64_t q_ld,
+                    const float* dev_temperature, const double* dev_uniforms, int32_t* dev_n_acc, int32_t* dev_next,
+                    float* dev_p, void* dev_ws, int64_t ws_bytes, int32_t* dev_status, void* stream) {
+  return guard(MK_ERR_ARG, [&] {
+    const char* who = "verify_draft";
+    const mkb::ActType t = act_type(type, true, who);
+    if (n_req < 0 || V <= 0 || V > kMaxVocab || n_rows < n_req) throw mkb::ArgError("verify_draft: bad shape");
+    if (ld < V || (dev_q && q_ld < V)) throw mkb::ArgError("verify_draft: rows overlap (a stride is shorter than its row)");
+    if (ws_bytes < mkb::verify_workspace(n_rows, V)) throw mkb::ArgError("verify_draft: workspace too small");
+    if (n_req > kMaxReq) throw mkb::ArgError("verify_draft: too many requests");
+    if (n_req == 0) return;
+    check_dev({{dev_logits, act_size(t), "dev_logits"}, {dev_row_off, 4, "dev_row_off"},
+               {dev_draft, 4, "dev_draft", n_rows == n_req}, {dev_q, 4, "dev_q", true},
+               {dev_temperature, 4, "dev_temperature"}, {dev_uniforms, 8, "dev_uniforms"}, {dev_n_acc, 4, "dev_n_acc"},
+               {dev_next, 4, "dev_next"}, {dev_p, 4, "dev_p", true}, {dev_ws, 16, "dev_ws"},
+               {dev_status, 4, "dev_status", true}}, who);
+    mkb::VerifyArgs a{dev_logits, ld, n_rows, V, n_req, dev_row_off, dev_draft, dev_q, q_ld, dev_temperature,
+                      dev_uniforms, dev_n_acc, dev_next, dev_p, dev_ws, dev_status};
+    mkb::cuda_check(static_cast<cudaError_t>(mkb::launch_verify_draft(a, t, current_sms(), as_stream(stream))), who);
   });
 }
 

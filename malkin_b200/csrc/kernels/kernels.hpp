@@ -237,4 +237,57 @@ void launch_accept(const AcceptReq* reqs, int n_req, const float* cand_v, const 
                    const int32_t* chain, const int32_t* alt, const float* q_p, const int32_t* q_id, const int32_t* q_n,
                    const double* uniforms, int n_ctx, AcceptOut* out, int32_t* from, int32_t* to, int32_t* count,
                    cudaStream_t s);
+
+// ---- serving operators on caller buffers (norm_rope.cu, attn_prompt.cu, attn_shared.cu, verify.cu) ----
+// The launchers only queue work: no allocation, no synchronization. Index tables live on the device; the kernels check
+// every index they follow, skip what is out of range and record the first such code in *status (nullable).
+enum class ActType { f32, f16, bf16 };
+constexpr int kStatusBadIndex = -1;  // MK_ERR_ARG: an index table points outside its buffer
+constexpr int kStatusTimeout = -7;   // MK_ERR_TIMEOUT: a bounded wait ran out
+
+struct NormRopeArgs {
+  const void* qkv;  // [n][ld]: q heads | k heads | v heads
+  int64_t ld;
+  int n, H, KV;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  const float* rope;  // [n_pos][cos D/2 | sin D/2]
+  int n_pos;
+  const int32_t* pos;
+  void* q;  // [n][q_ld]
+  int64_t q_ld;
+  void* k;  // nullable
+  int64_t k_ld;
+  int8_t* kc;  // int8 cache of one layer [KV][n_rows][D] (nullable)
+  int8_t* vc;
+  float* ks;
+  float* vs;
+  int64_t n_rows;
+  const int32_t* kv_at;
+  int* status;
+};
+void launch_qk_norm_rope(const NormRopeArgs& a, ActType type, int D, int sms, cudaStream_t s);
+
+struct VerifyArgs {
+  const void* logits;  // [n_rows][ld]
+  int64_t ld;
+  int n_rows, V, n_req;
+  const int32_t* row_off;  // [n_req + 1]
+  const int32_t* draft;    // [n_rows - n_req]
+  const float* q;          // [n_rows - n_req][q_ld] (nullable)
+  int64_t q_ld;
+  const float* temperature;  // [n_req]
+  const double* u;           // [n_rows]
+  int32_t* n_acc;
+  int32_t* next;
+  float* p;  // [n_rows - n_req] (nullable)
+  void* ws;
+  int* status;
+};
+// Bytes of VerifyArgs::ws.
+int64_t verify_workspace(int n_rows, int V);
+// 0, or the CUDA error of a launch that could not be queued.
+int launch_verify_draft(const VerifyArgs& a, ActType type, int sms, cudaStream_t s);
+
 }  // namespace mkb

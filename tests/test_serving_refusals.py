@@ -1,0 +1,58 @@
+"""Refusals of the serving operators: every one is made before a device is looked at, so they are tested without a GPU."""
+import pytest
+
+F32, F16, BF16, Q8 = 0, 1, 30, 8
+P = 1 << 20  # stands for a device pointer: the calls below are refused before it is looked at
+
+
+def refused(mk, f, *a, code=None, text=None, **k):
+    with pytest.raises(mk.MalkinError) as e:
+        f(*a, **k)
+    assert e.value.code == (mk.MK_ERR_ARG if code is None else code), str(e.value)
+    if text:
+        assert text in str(e.value)
+
+
+def norm(mk, **k):
+    a = dict(type_=BF16, dev_qkv=P, ld=6 * 128, n=2, H=2, KV=2, D=128, dev_q_norm=P, dev_k_norm=P, eps=1e-6, dev_rope=P,
+             n_pos=4, dev_pos=P, dev_q=P, q_ld=256, dev_k=P, k_ld=256)
+    a.update(k)
+    mk.qk_norm_rope(**a)
+
+
+@pytest.mark.parametrize("change", [
+    dict(type_=Q8), dict(type_=99), dict(n=-1), dict(H=0), dict(KV=0), dict(H=5000), dict(D=96), dict(D=0),
+    dict(n_pos=0), dict(eps=-1.0), dict(eps=float("nan")), dict(ld=6 * 128 - 1), dict(q_ld=255), dict(k_ld=255),
+    dict(dev_kc=P, dev_vc=P, dev_ks=P, dev_vs=P, n_rows=0, dev_kv_at=P),
+    dict(dev_kc=P, dev_vc=P, dev_ks=P, dev_vs=P, n_rows=4), dict(dev_kc=P, n_rows=4, dev_kv_at=P),
+    dict(dev_qkv=0), dict(dev_qkv=P + 1), dict(dev_pos=P + 2), dict(dev_q=0), dict(type_=F32, dev_q=P + 2)])
+def test_norm_rope_refuses(mk, change):
+    refused(mk, norm, mk, **change)
+
+
+def verify(mk, **k):
+    a = dict(type_=F32, dev_logits=P, ld=100, n_rows=6, V=100, n_req=2, dev_row_off=P, dev_draft=P, dev_q=P, q_ld=100,
+             dev_temperature=P, dev_uniforms=P, dev_n_acc=P, dev_next=P, dev_p=P, dev_ws=P, ws_bytes=1 << 20)
+    a.update(k)
+    mk.verify_draft(**a)
+
+
+@pytest.mark.parametrize("change", [
+    dict(type_=Q8), dict(V=0), dict(V=(1 << 27) + 1, ld=1 << 28, q_ld=1 << 28), dict(n_req=-1), dict(n_rows=1),
+    dict(ld=99), dict(q_ld=99), dict(ws_bytes=0), dict(dev_ws=P + 8), dict(dev_logits=0), dict(dev_logits=P + 2),
+    dict(dev_uniforms=P + 4), dict(dev_row_off=0), dict(dev_draft=0), dict(dev_next=0)])
+def test_verify_refuses(mk, change):
+    refused(mk, verify, mk, **change)
+
+
+def test_workspace_sizes(mk):
+    assert mk.verify_draft_workspace(0, 0, 1) > 0
+    assert mk.verify_draft_workspace(9, 1, 151936) >= 9 * 38 * 16
+    refused(mk, mk.verify_draft_workspace, 1, 1, 0)
+    refused(mk, mk.verify_draft_workspace, -1, 0, 10)
+
+
+def test_nothing_to_do(mk):
+    """No tokens, no requests: nothing is looked at."""
+    norm(mk, n=0)
+    verify(mk, n_req=0, n_rows=0)
