@@ -360,6 +360,18 @@ int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int
                     void* dev_q, int64_t q_ld, void* dev_k, int64_t k_ld, int8_t* dev_kc, int8_t* dev_vc, float* dev_ks,
                     float* dev_vs, int64_t n_rows, const int32_t* dev_kv_at, int32_t* dev_status, void* stream);
 
+/* Causal attention over packed prompts (Model::attention of a whole prompt batch, model.cpp:204-247, on 16-bit q, k, v
+ * instead of the int8 cache): rows dev_off[s] .. dev_off[s + 1] - 1 of the buffers are sequence s (n_seq + 1 ascending
+ * entries, the last at most n; a sequence may be empty), row i attends to rows 0 .. i of its sequence. Query head h reads
+ * KV head h / (H / KV). dev_q and dev_out: n rows of H x D, dev_k and dev_v: n rows of KV x D, each with its own stride;
+ * type MK_TYPE_F16 or MK_TYPE_BF16, D 64 or 128, buffers 16-byte aligned, strides multiples of 8, scale > 0.
+ * Rows of no sequence are left as they were, and what masked rows hold (later tokens, other sequences, NaN or infinities
+ * among them) does not reach an output. Offsets that descend or leave 0 .. n: that sequence's rows are left as they were
+ * and MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside the kernel ran out, the outputs are not valid. */
+int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* dev_k, int64_t k_ld, const void* dev_v,
+                        int64_t v_ld, int n, int n_seq, const int32_t* dev_off, int H, int KV, int D, float scale,
+                        void* dev_out, int64_t out_ld, int32_t* dev_status, void* stream);
+
 /* Verification of drafted tokens over the whole vocabulary: Engine::accept_sampled / accept_greedy's chain and
  * Sampler::verify / draw (engine.cpp:441-507, sampler.cpp:64-97) with softmax(logits / temperature) of all V tokens
  * where mk_accept works on at most MK_MAX_TOPK candidates (no top-k, top-p or min-p here).

@@ -206,7 +206,7 @@ EXPORTS = ("mk_last_error", "mk_version", "mk_synth_gguf", "mk_init", "mk_nccl_u
            "mk_matmul", "mk_matmul_noalloc", "mk_block_dots", "mk_quantize_i8", "mk_silu_mul", "mk_attention",
            "mk_engine_create", "mk_engine_destroy", "mk_engine_submit", "mk_engine_step", "mk_engine_events",
            "mk_engine_busy", "mk_engine_cancel", "mk_engine_stats", "mk_engine_perplexity", "mk_qk_norm_rope",
-           "mk_verify_draft_workspace", "mk_verify_draft")
+           "mk_verify_draft_workspace", "mk_verify_draft", "mk_attention_prompt")
 
 
 def version() -> str:
@@ -524,6 +524,19 @@ def qk_norm_rope(type_: int, dev_qkv: int, ld: int, n: int, H: int, KV: int, D: 
     _check(lib.mk_qk_norm_rope(type_, dev_qkv, ld, n, H, KV, D, dev_q_norm, dev_k_norm, eps, dev_rope, n_pos, dev_pos,
                                dev_q, q_ld, dev_k or None, k_ld, dev_kc or None, dev_vc or None, dev_ks or None,
                                dev_vs or None, n_rows, dev_kv_at or None, dev_status or None, stream or None))
+
+
+lib.mk_attention_prompt.argtypes = [ctypes.c_int, _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                                    ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                    ctypes.c_float, _vp, ctypes.c_int64, _vp, _vp]
+
+
+def attention_prompt(type_: int, dev_q: int, q_ld: int, dev_k: int, k_ld: int, dev_v: int, v_ld: int, n: int,
+                     n_seq: int, dev_off: int, H: int, KV: int, D: int, scale: float, dev_out: int, out_ld: int,
+                     dev_status: int = 0, stream: int = 0) -> None:
+    """Causal grouped-query attention over packed prompts (mk_attention_prompt). type_: TYPE_F16 or TYPE_BF16."""
+    _check(lib.mk_attention_prompt(type_, dev_q, q_ld, dev_k, k_ld, dev_v, v_ld, n, n_seq, dev_off, H, KV, D, scale,
+                                   dev_out, out_ld, dev_status or None, stream or None))
 
 
 def verify_draft_workspace(n_rows: int, n_req: int, V: int) -> int:

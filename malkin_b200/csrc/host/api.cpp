@@ -100,6 +100,13 @@ mkb::ActType act_type(int type, bool with_f32, const char* who) {
 }
 size_t act_size(mkb::ActType t) { return t == mkb::ActType::f32 ? 4 : 2; }
 
+void check_heads(int H, int KV, int D, float scale, const char* who) {
+  if (H <= 0 || KV <= 0 || H > kMaxHeads || H % KV) throw mkb::ArgError(std::string(who) + ": H must be a multiple of KV");
+  if (D == 256) throw mkb::UnsupportedError(std::string(who) + ": head width 256 (mk_attention takes it)");
+  if (D != 64 && D != 128) throw mkb::ArgError(std::string(who) + ": head width must be 64 or 128");
+  if (!(scale > 0.0f) || !std::isfinite(scale)) throw mkb::ArgError(std::string(who) + ": scale must be positive");
+}
+
 struct DevArg {
   const void* p;
   size_t align;
@@ -589,6 +596,27 @@ int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int
                         dev_k, k_ld, dev_kc, dev_vc, dev_ks, dev_vs, n_rows, dev_kv_at, dev_status};
     mkb::launch_qk_norm_rope(a, t, D, current_sms(), as_stream(stream));
     mkb::cuda_check(cudaGetLastError(), who);
+  });
+}
+
+int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* dev_k, int64_t k_ld, const void* dev_v,
+                        int64_t v_ld, int n, int n_seq, const int32_t* dev_off, int H, int KV, int D, float scale,
+                        void* dev_out, int64_t out_ld, int32_t* dev_status, void* stream) {
+  return guard(MK_ERR_ARG, [&] {
+    const char* who = "attention_prompt";
+    const mkb::ActType t = act_type(type, false, who);
+    check_heads(H, KV, D, scale, who);
+    if (n < 0 || n_seq < 0 || n_seq > kMaxReq) throw mkb::ArgError("attention_prompt: bad shape");
+    const int64_t qw = static_cast<int64_t>(H) * D, kw = static_cast<int64_t>(KV) * D;
+    if (q_ld < qw || k_ld < kw || v_ld < kw || out_ld < qw)
+      throw mkb::ArgError("attention_prompt: rows overlap (a stride is shorter than its row)");
+    if (q_ld % 8 || k_ld % 8 || v_ld % 8 || out_ld % 8)
+      throw mkb::ArgError("attention_prompt: strides must be multiples of 8");
+    if (n == 0 || n_seq == 0) return;
+    check_dev({{dev_q, 16, "dev_q"}, {dev_k, 16, "dev_k"}, {dev_v, 16, "dev_v"}, {dev_off, 4, "dev_off"},
+               {dev_out, 16, "dev_out"}, {dev_status, 4, "dev_status", true}}, who);
+    mkb::PromptArgs a{dev_q, q_ld, dev_k, k_ld, dev_v, v_ld, n, n_seq, dev_off, H, KV, scale, dev_out, out_ld, dev_status};
+    mkb::cuda_check(static_cast<cudaError_t>(mkb::launch_attention_prompt(a, t, D, as_stream(stream))), who);
   });
 }
 

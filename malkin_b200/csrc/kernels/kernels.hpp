@@ -290,4 +290,22 @@ int64_t verify_workspace(int n_rows, int V);
 // 0, or the CUDA error of a launch that could not be queued.
 int launch_verify_draft(const VerifyArgs& a, ActType type, int sms, cudaStream_t s);
 
+struct PromptArgs {
+  const void* q;  // [n][q_ld], heads D apart
+  int64_t q_ld;
+  const void* k;
+  int64_t k_ld;
+  const void* v;
+  int64_t v_ld;
+  int n, n_seq;
+  const int32_t* off;  // [n_seq + 1]
+  int H, KV;
+  float scale;
+  void* out;
+  int64_t out_ld;
+  int* status;
+};
+// 0 or a CUDA error. D 64 or 128; buffers 16-byte aligned, strides multiples of 8.
+int launch_attention_prompt(const PromptArgs& a, ActType type, int D, cudaStream_t s);
+
 }  // namespace mkb

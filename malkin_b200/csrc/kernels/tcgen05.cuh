@@ -41,6 +41,20 @@ __device__ __forceinline__ uint32_t umma_idesc_f16_f32(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Descriptors of operand tiles with 128-byte swizzle (rows of 128 bytes, 8 rows to a 1024-byte atom, as TMA writes them):
+// K-major (a row holds 64 16-bit values along K; sbo: bytes between 8-row groups) and MN-major (a row holds 64 values
+// along M or N; lbo: bytes between blocks of 64 of them, sbo: bytes between groups of 8 along K). Layout type 2 at bit 61.
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return umma_desc_kmajor(saddr, lbo, sbo) | (static_cast<uint64_t>(2) << 61);
+}
+
+// kind::f16 with f32 accumulators: fp16 (fmt 0) or bf16 (fmt 1) A and B; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t umma_idesc_16(int fmt, bool b_mn, int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(fmt) << 7) | (static_cast<uint32_t>(fmt) << 10) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+
 // D[tmem] (+)= A[smem] x B[smem]^T (int8), issued by one thread; acc = 0 overwrites D.
 __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                           uint32_t acc) {
@@ -119,6 +133,23 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+// 2^x, the hardware approximation (denormal results flush to 0).
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Register split of a warpgroup (every warp of the group executes it; the groups' shares sum to at most the launch's).
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

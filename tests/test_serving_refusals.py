@@ -30,6 +30,26 @@ def test_norm_rope_refuses(mk, change):
     refused(mk, norm, mk, **change)
 
 
+def prompt(mk, **k):
+    a = dict(type_=BF16, dev_q=P, q_ld=512, dev_k=P, k_ld=256, dev_v=P, v_ld=256, n=10, n_seq=2, dev_off=P, H=4, KV=2,
+             D=128, scale=0.1, dev_out=P, out_ld=512)
+    a.update(k)
+    mk.attention_prompt(**a)
+
+
+@pytest.mark.parametrize("change", [
+    dict(type_=F32), dict(type_=Q8), dict(H=0), dict(KV=0), dict(H=3), dict(D=96), dict(n=-1), dict(n_seq=-1),
+    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q_ld=511),
+    dict(q_ld=516), dict(k_ld=255), dict(v_ld=260), dict(out_ld=504), dict(dev_q=P + 8), dict(dev_out=P + 2),
+    dict(dev_k=0), dict(dev_off=P + 1)])
+def test_prompt_refuses(mk, change):
+    refused(mk, prompt, mk, **change)
+
+
+def test_prompt_width_256_is_unsupported(mk):
+    refused(mk, prompt, mk, D=256, q_ld=1024, k_ld=512, v_ld=512, out_ld=1024, code=mk.MK_ERR_UNSUPPORTED)
+
+
 def verify(mk, **k):
     a = dict(type_=F32, dev_logits=P, ld=100, n_rows=6, V=100, n_req=2, dev_row_off=P, dev_draft=P, dev_q=P, q_ld=100,
              dev_temperature=P, dev_uniforms=P, dev_n_acc=P, dev_next=P, dev_p=P, dev_ws=P, ws_bytes=1 << 20)
@@ -56,3 +76,5 @@ def test_nothing_to_do(mk):
     """No tokens, no requests: nothing is looked at."""
     norm(mk, n=0)
     verify(mk, n_req=0, n_rows=0)
+    prompt(mk, n=0)
+    prompt(mk, n_seq=0)
