@@ -372,6 +372,30 @@ int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* d
                         int64_t v_ld, int n, int n_seq, const int32_t* dev_off, int H, int KV, int D, float scale,
                         void* dev_out, int64_t out_ld, int32_t* dev_status, void* stream);
 
+/* Tree-masked GQA attention of a decoding batch whose requests share prefixes (Model::attention + kern::attend_gqa,
+ * model.cpp:204-247, kernels_avx512.cpp:229-307; malkin keeps a copy of the prefix in every slot and reads each). The cache
+ * and the per-token tables are mk_attention's: dev_k / dev_v int8 [KV][n_rows][D], dev_ks / dev_vs float [KV][n_rows];
+ * token t attends to rows dev_kv_base[t] .. + dev_n_keys[t] - 1 and to the rows dev_anc[dev_anc_off[t] ..
+ * dev_anc_off[t + 1]) relative to dev_kv_base[t] (dev_anc_off NULL: none; n_anc entries). In addition the tokens
+ * dev_group_off[g] .. dev_group_off[g + 1] - 1 (n_groups + 1 ascending entries; a token may be in no group) attend to the
+ * rows dev_prefix_base[g] .. + dev_prefix_len[g] - 1, read once for up to 128 / (H / KV) of them. All of a token's keys are
+ * in one softmax; a token without any gives zeros. Consecutive tokens with the same dev_kv_base share one pass over its
+ * rows, so a request's tokens belong next to each other. n_groups = 0 is allowed.
+ * dev_q and dev_out: n rows of H x D, q_ld / out_ld apart, type MK_TYPE_F16 or MK_TYPE_BF16; D 64 or 128, H / KV at most
+ * 128, scale > 0; dev_q, dev_k, dev_v, dev_out and dev_ws 16-byte aligned, strides multiples of 8.
+ * Rows outside the tables are not looked at, nor are their scales. A group or token whose rows leave the cache, or a group
+ * whose tokens leave 0 .. n, has none of those keys, a token whose ancestors do loses them from the first such one on, and
+ * MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside a kernel ran out, the outputs are not valid.
+ * dev_ws: mk_attention_shared_workspace(n, H, KV, D, n_groups) bytes (negative: bad shape or no device; about
+ * 16 n H (D + 2) bytes and 256 x 128 x (D + 2) x 4 for the largest device). */
+int64_t mk_attention_shared_workspace(int n, int H, int KV, int D, int n_groups);
+int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H, int KV, int D, float scale,
+                        const int8_t* dev_k, const int8_t* dev_v, const float* dev_ks, const float* dev_vs,
+                        int64_t n_rows, int n_groups, const int32_t* dev_group_off, const int32_t* dev_prefix_base,
+                        const int32_t* dev_prefix_len, const int32_t* dev_kv_base, const int32_t* dev_n_keys,
+                        const int32_t* dev_anc_off, const int32_t* dev_anc, int n_anc, void* dev_out, int64_t out_ld,
+                        void* dev_ws, int64_t ws_bytes, int32_t* dev_status, void* stream);
+
 /* Verification of drafted tokens over the whole vocabulary: Engine::accept_sampled / accept_greedy's chain and
  * Sampler::verify / draw (engine.cpp:441-507, sampler.cpp:64-97) with softmax(logits / temperature) of all V tokens
  * where mk_accept works on at most MK_MAX_TOPK candidates (no top-k, top-p or min-p here).

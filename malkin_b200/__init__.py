@@ -206,7 +206,8 @@ EXPORTS = ("mk_last_error", "mk_version", "mk_synth_gguf", "mk_init", "mk_nccl_u
            "mk_matmul", "mk_matmul_noalloc", "mk_block_dots", "mk_quantize_i8", "mk_silu_mul", "mk_attention",
            "mk_engine_create", "mk_engine_destroy", "mk_engine_submit", "mk_engine_step", "mk_engine_events",
            "mk_engine_busy", "mk_engine_cancel", "mk_engine_stats", "mk_engine_perplexity", "mk_qk_norm_rope",
-           "mk_verify_draft_workspace", "mk_verify_draft", "mk_attention_prompt")
+           "mk_verify_draft_workspace", "mk_verify_draft", "mk_attention_prompt",
+           "mk_attention_shared_workspace", "mk_attention_shared")
 
 
 def version() -> str:
@@ -537,6 +538,35 @@ def attention_prompt(type_: int, dev_q: int, q_ld: int, dev_k: int, k_ld: int, d
     """Causal grouped-query attention over packed prompts (mk_attention_prompt). type_: TYPE_F16 or TYPE_BF16."""
     _check(lib.mk_attention_prompt(type_, dev_q, q_ld, dev_k, k_ld, dev_v, v_ld, n, n_seq, dev_off, H, KV, D, scale,
                                    dev_out, out_ld, dev_status or None, stream or None))
+
+
+lib.mk_attention_shared_workspace.argtypes = [ctypes.c_int] * 5
+lib.mk_attention_shared_workspace.restype = ctypes.c_int64
+lib.mk_attention_shared.argtypes = [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                    ctypes.c_int, ctypes.c_float, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int, _vp,
+                                    _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int64, _vp,
+                                    ctypes.c_int64, _vp, _vp]
+
+
+def attention_shared_workspace(n: int, H: int, KV: int, D: int, n_groups: int) -> int:
+    """Workspace bytes of attention_shared on the current device."""
+    b = lib.mk_attention_shared_workspace(n, H, KV, D, n_groups)
+    if b < 0:
+        raise MalkinError(int(b), lib.mk_last_error().decode())
+    return b
+
+
+def attention_shared(type_: int, dev_q: int, q_ld: int, n: int, H: int, KV: int, D: int, scale: float, dev_k: int,
+                     dev_v: int, dev_ks: int, dev_vs: int, n_rows: int, n_groups: int, dev_group_off: int,
+                     dev_prefix_base: int, dev_prefix_len: int, dev_kv_base: int, dev_n_keys: int, dev_anc_off: int,
+                     dev_anc: int, n_anc: int, dev_out: int, out_ld: int, dev_ws: int, ws_bytes: int,
+                     dev_status: int = 0, stream: int = 0) -> None:
+    """Tree-masked attention over the int8 cache with prefixes shared by groups of requests (mk_attention_shared).
+    type_: TYPE_F16 or TYPE_BF16."""
+    _check(lib.mk_attention_shared(type_, dev_q, q_ld, n, H, KV, D, scale, dev_k, dev_v, dev_ks, dev_vs, n_rows,
+                                   n_groups, dev_group_off or None, dev_prefix_base or None, dev_prefix_len or None,
+                                   dev_kv_base, dev_n_keys, dev_anc_off or None, dev_anc or None, n_anc, dev_out,
+                                   out_ld, dev_ws, ws_bytes, dev_status or None, stream or None))
 
 
 def verify_draft_workspace(n_rows: int, n_req: int, V: int) -> int:

@@ -107,6 +107,12 @@ void check_heads(int H, int KV, int D, float scale, const char* who) {
   if (!(scale > 0.0f) || !std::isfinite(scale)) throw mkb::ArgError(std::string(who) + ": scale must be positive");
 }
 
+void check_shared(int n, int H, int KV, int n_groups, const char* who) {
+  if (n < 0 || n_groups < 0 || n_groups > kMaxReq || n > kMaxReq)
+    throw mkb::ArgError(std::string(who) + ": bad shape");
+  if (H / KV > 128) throw mkb::ArgError(std::string(who) + ": at most 128 query heads per KV head");
+}
+
 struct DevArg {
   const void* p;
   size_t align;
@@ -617,6 +623,51 @@ int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* d
                {dev_out, 16, "dev_out"}, {dev_status, 4, "dev_status", true}}, who);
     mkb::PromptArgs a{dev_q, q_ld, dev_k, k_ld, dev_v, v_ld, n, n_seq, dev_off, H, KV, scale, dev_out, out_ld, dev_status};
     mkb::cuda_check(static_cast<cudaError_t>(mkb::launch_attention_prompt(a, t, D, as_stream(stream))), who);
+  });
+}
+
+int64_t mk_attention_shared_workspace(int n, int H, int KV, int D, int n_groups) {
+  int64_t bytes = -1;
+  const int rc = guard(MK_ERR_ARG, [&] {
+    const char* who = "attention_shared_workspace";
+    check_heads(H, KV, D, 1.0f, who);
+    check_shared(n, H, KV, n_groups, who);
+    bytes = mkb::attention_shared_workspace(n, H, KV, D, n_groups, current_sms());
+  });
+  return rc == MK_OK ? bytes : rc;
+}
+
+int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H, int KV, int D, float scale,
+                        const int8_t* dev_k, const int8_t* dev_v, const float* dev_ks, const float* dev_vs,
+                        int64_t n_rows, int n_groups, const int32_t* dev_group_off, const int32_t* dev_prefix_base,
+                        const int32_t* dev_prefix_len, const int32_t* dev_kv_base, const int32_t* dev_n_keys,
+                        const int32_t* dev_anc_off, const int32_t* dev_anc, int n_anc, void* dev_out, int64_t out_ld,
+                        void* dev_ws, int64_t ws_bytes, int32_t* dev_status, void* stream) {
+  return guard(MK_ERR_ARG, [&] {
+    const char* who = "attention_shared";
+    const mkb::ActType t = act_type(type, false, who);
+    check_heads(H, KV, D, scale, who);
+    check_shared(n, H, KV, n_groups, who);
+    if (n_rows <= 0 || n_anc < 0) throw mkb::ArgError("attention_shared: bad shape");
+    const int64_t qw = static_cast<int64_t>(H) * D;
+    if (q_ld < qw || out_ld < qw)
+      throw mkb::ArgError("attention_shared: rows overlap (a stride is shorter than its row)");
+    if (q_ld % 8 || out_ld % 8) throw mkb::ArgError("attention_shared: strides must be multiples of 8");
+    if (n == 0) return;
+    const bool anc = dev_anc_off && n_anc > 0;
+    check_dev({{dev_q, 16, "dev_q"}, {dev_k, 16, "dev_k"}, {dev_v, 16, "dev_v"}, {dev_ks, 4, "dev_ks"},
+               {dev_vs, 4, "dev_vs"}, {dev_group_off, 4, "dev_group_off", n_groups == 0},
+               {dev_prefix_base, 4, "dev_prefix_base", n_groups == 0}, {dev_prefix_len, 4, "dev_prefix_len", n_groups == 0},
+               {dev_kv_base, 4, "dev_kv_base"}, {dev_n_keys, 4, "dev_n_keys"}, {dev_anc_off, 4, "dev_anc_off", true},
+               {anc ? dev_anc : nullptr, 4, "dev_anc", !anc}, {dev_out, 16, "dev_out"}, {dev_ws, 16, "dev_ws"},
+               {dev_status, 4, "dev_status", true}}, who);
+    const int sms = current_sms();
+    if (ws_bytes < mkb::attention_shared_workspace(n, H, KV, D, n_groups, sms))
+      throw mkb::ArgError("attention_shared: workspace too small");
+    mkb::SharedArgs a{dev_q, q_ld, n, H, KV, scale, dev_k, dev_v, dev_ks, dev_vs, n_rows, n_groups, dev_group_off,
+                      dev_prefix_base, dev_prefix_len, dev_kv_base, dev_n_keys, dev_anc_off, dev_anc, n_anc, dev_out,
+                      out_ld, dev_status};
+    mkb::cuda_check(static_cast<cudaError_t>(mkb::launch_attention_shared(a, t, D, dev_ws, sms, as_stream(stream))), who);
   });
 }
 

@@ -2,7 +2,7 @@
 //
 // Row i of a sequence: out_i = sum_{j <= i} p_j v_j / sum p_j, p_j = exp(scale q_i k_j - m). One pass over the keys with
 // the running maximum and sum of the softmax per row (fp32), S = Q K^T and O += P V on tcgen05 with both accumulators in
-// TMEM. P is rounded to the operands' type (half a step of it, 2^-9 or 2^-12, on each weight; the sum of the weights is
+// TMEM. P is rounded to the operands' type (half a step of it, 2^-8 or 2^-11, of each weight; the sum of the weights is
 // taken before that rounding): tcgen05 has no wider A operand at this rate, and the errors of a row's weights average out.
 //
 // A CTA takes 256 rows of one head as two tiles of 128, so each K / V tile read from L2 feeds two tiles, and one tile's

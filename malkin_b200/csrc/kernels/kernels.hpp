@@ -308,4 +308,31 @@ struct PromptArgs {
 // 0 or a CUDA error. D 64 or 128; buffers 16-byte aligned, strides multiples of 8.
 int launch_attention_prompt(const PromptArgs& a, ActType type, int D, cudaStream_t s);
 
+struct SharedArgs {
+  const void* q;  // [n][q_ld]
+  int64_t q_ld;
+  int n, H, KV;
+  float scale;
+  const int8_t* k;  // [KV][n_rows][D]
+  const int8_t* v;
+  const float* ks;  // [KV][n_rows]
+  const float* vs;
+  int64_t n_rows;
+  int n_groups;
+  const int32_t* group_off;  // [n_groups + 1] token ranges
+  const int32_t* prefix_base;
+  const int32_t* prefix_len;
+  const int32_t* kv_base;  // [n]
+  const int32_t* n_keys;   // [n]
+  const int32_t* anc_off;  // [n + 1] (nullable)
+  const int32_t* anc;
+  int n_anc;
+  void* out;
+  int64_t out_ld;
+  int* status;
+};
+int64_t attention_shared_workspace(int n, int H, int KV, int D, int n_groups, int sms);
+// 0 or a CUDA error. D 64 or 128, H / KV at most 128; q, k, v and out 16-byte aligned, strides multiples of 8.
+int launch_attention_shared(const SharedArgs& a, ActType type, int D, void* ws, int sms, cudaStream_t s);
+
 }  // namespace mkb

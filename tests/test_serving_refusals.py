@@ -50,6 +50,30 @@ def test_prompt_width_256_is_unsupported(mk):
     refused(mk, prompt, mk, D=256, q_ld=1024, k_ld=512, v_ld=512, out_ld=1024, code=mk.MK_ERR_UNSUPPORTED)
 
 
+def shared(mk, **k):
+    a = dict(type_=F16, dev_q=P, q_ld=512, n=6, H=4, KV=2, D=128, scale=0.1, dev_k=P, dev_v=P, dev_ks=P, dev_vs=P,
+             n_rows=100, n_groups=1, dev_group_off=P, dev_prefix_base=P, dev_prefix_len=P, dev_kv_base=P, dev_n_keys=P,
+             dev_anc_off=P, dev_anc=P, n_anc=3, dev_out=P, out_ld=512, dev_ws=P, ws_bytes=1 << 40)
+    a.update(k)
+    mk.attention_shared(**a)
+
+
+@pytest.mark.parametrize("change", [
+    dict(type_=F32), dict(H=5), dict(H=0), dict(D=80), dict(n=-1), dict(n_groups=-1), dict(n_rows=0), dict(n_anc=-1),
+    dict(H=258, KV=2, q_ld=258 * 128, out_ld=258 * 128), dict(scale=0.0), dict(scale=float("nan")), dict(q_ld=508),
+    dict(q_ld=515), dict(out_ld=511), dict(dev_q=P + 8), dict(dev_k=P + 4), dict(dev_out=P + 4), dict(dev_ws=P + 8),
+    dict(dev_ks=0), dict(dev_group_off=0), dict(dev_kv_base=0), dict(dev_n_keys=P + 1), dict(dev_anc=0)])
+def test_shared_refuses(mk, change):
+    refused(mk, shared, mk, **change)
+
+
+def test_shared_width_256_is_unsupported(mk):
+    refused(mk, shared, mk, D=256, q_ld=1024, out_ld=1024, code=mk.MK_ERR_UNSUPPORTED)
+    refused(mk, mk.attention_shared_workspace, 4, 4, 2, 256, 1, code=mk.MK_ERR_UNSUPPORTED)
+    refused(mk, mk.attention_shared_workspace, 4, 3, 2, 128, 1)
+    refused(mk, mk.attention_shared_workspace, -4, 4, 2, 128, 1)
+
+
 def verify(mk, **k):
     a = dict(type_=F32, dev_logits=P, ld=100, n_rows=6, V=100, n_req=2, dev_row_off=P, dev_draft=P, dev_q=P, q_ld=100,
              dev_temperature=P, dev_uniforms=P, dev_n_acc=P, dev_next=P, dev_p=P, dev_ws=P, ws_bytes=1 << 20)
@@ -78,3 +102,4 @@ def test_nothing_to_do(mk):
     verify(mk, n_req=0, n_rows=0)
     prompt(mk, n=0)
     prompt(mk, n_seq=0)
+    shared(mk, n=0)
