@@ -12,7 +12,10 @@
 //   k_shared_join     a warp per (token, head): joins its partial triples and the ancestors' few keys
 //
 // int8 values are exact in both 16-bit types. Row scales of K (with scale and log2 e) multiply the scores, those of V the
-// weights; weights are rounded to bf16 (2^-8 of each; the range of fp16 would not hold weight x scale).
+// weights. P V is in fp16 whatever q's type: a weight x scale is rounded by 2^-11 of itself (bf16 would lose 2^-8, which is
+// what an fp16 output would then be off by). To stay in fp16's range the row's reference exponent is not the largest score
+// but that plus the exponent of the block's largest V scale, less 6: products are at most 2^15, and full precision reaches
+// down to 2^-20 of the largest. Sums and outputs carry the same reference, so it cancels.
 // Bound: HBM for one tile of rows a group (128 rows: 65.5 kFLOP against 264 bytes a key and head, the machine's balance),
 // the tensor pipe and the conversion above that.
 #include <cuda_bf16.h>
@@ -38,7 +41,9 @@ constexpr int kPlanThreads = 1024;
 constexpr int kAttendThreads = 384;  // warpgroups: softmax, conversion, MMA (one thread)
 constexpr int kRegsSoftmax = 128, kRegsConvert = 88, kRegsMma = 24;  // sum: 3 x the 80 of the launch
 constexpr int kCtasPerSm = 2;
-constexpr float kRaiseMax = 8.0f;  // a row's maximum is raised when it grew by more (exponents of 2)
+constexpr float kRaiseMax = 8.0f;   // a row's reference is raised when it is to grow by more (exponents of 2)
+constexpr float kHeadroom = 6.0f;   // of it below the largest weight x scale
+constexpr int kLeastExp = -40;      // of a block's largest V scale: blocks of zeros must not push the sums out of range
 
 struct Tile {
   int32_t t0, nt;      // tokens
@@ -60,7 +65,7 @@ struct SharedWs {  // the workspace's parts
   int32_t* tok_pre;  // [n] tile of the token's prefix, -1: none
   int32_t* tok_own;  // [n]
   int32_t* group_tile;  // [n_groups]
-  float2* ml;        // [rows] maximum (exponent of 2), sum
+  float2* ml;        // [rows] reference (exponent of 2), sum
   float* o;          // [rows][D]
   int64_t rows;
   int prefix_tiles;  // room for tiles over prefixes
@@ -368,6 +373,7 @@ struct SharedSmall {
   uint64_t q_full, q_empty, full[2], empty[2], s_full[2], p_full[2], pv_done, o_free;
   float ks[2][kBlock];  // K scale x scale x log2 e
   float vs[2][kBlock];
+  float vmax[2][2];         // largest finite |V scale| of each half of the block
   uint32_t tmem;
 };
 template <int D>
@@ -450,10 +456,13 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
             for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float big = fmaxf(sm->vmax[s][0], sm->vmax[s][1]);
+          const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, kLeastExp);
+          const float want = top + (static_cast<float>(e) - kHeadroom);
           float scale = 1.0f;
-          if (top > m && (m == -INFINITY || top - m > kRaiseMax)) {
-            scale = ex2_approx(m - top);
-            m = top;
+          if (want > m && (m == -INFINITY || want - m > kRaiseMax)) {
+            scale = ex2_approx(m - want);
+            m = want;
           }
           if (b > walk.b0 && __any_sync(0xffffffffu, scale != 1.0f)) {
             ok = mbar_wait_warp(&sm->pv_done, (gb - 1) & 1, st, kStatusTimeout);
@@ -488,8 +497,8 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
                 w0 = f2_make(j < left ? f2_lo(w0) : 0.0f, j + 1 < left ? f2_hi(w0) : 0.0f);
                 w1 = f2_make(j + 2 < left ? f2_lo(w1) : 0.0f, j + 3 < left ? f2_hi(w1) : 0.0f);
               }
-              p[i] = pack2<__nv_bfloat16>(f2_lo(w0), f2_hi(w0));
-              p[i + 1] = pack2<__nv_bfloat16>(f2_lo(w1), f2_hi(w1));
+              p[i] = pack2<__half>(f2_lo(w0), f2_hi(w0));
+              p[i + 1] = pack2<__half>(f2_lo(w1), f2_hi(w1));
             }
             tmem_st16(ts + 16 * c, p);
           }
@@ -595,6 +604,10 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
           len = more ? walk.x.len : 0;
         }
         (t < 64 ? sm->ks[s] : sm->vs[s])[t & 63] = sreg;
+        if (t >= 64) {
+          const float big = warp_max(fabsf(sreg) < INFINITY ? fabsf(sreg) : 0.0f);
+          if (lane == 0) sm->vmax[s][(t - 64) >> 5] = big;
+        }
 #pragma unroll
         for (int i = 0; i < L; ++i) {
           store_row(k_tile(s), i, kreg[i], T());
@@ -602,7 +615,7 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
         }
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-          store_row(v_tile(s), i, vreg[i], __nv_bfloat16());
+          store_row(v_tile(s), i, vreg[i], __half());
           vreg[i] = load_row(a.v, row0, len, nb, i);
         }
         sreg = load_scale(row0, len, nb);
@@ -615,7 +628,7 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
     if (warp == 8 && lane == 0) {
       // ---------------- MMA ----------------
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
-      constexpr uint32_t id_s = umma_idesc_16(fmt, false, kTileRows, kBlock), id_o = umma_idesc_16(1, true, kTileRows, D);
+      constexpr uint32_t id_s = umma_idesc_16(fmt, false, kTileRows, kBlock), id_o = umma_idesc_16(0, true, kTileRows, D);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity & 1, st, kStatusTimeout); };
       auto scores = [&](int s) {
         const uint32_t q = smem_addr(smem), k = smem_addr(k_tile(s));
