@@ -8,7 +8,7 @@
 //
 //   k_verify_rows  one CTA per (row, vocabulary chunk): maximum, its lowest index, and sum of exp((l - max) / T).
 //                  Bound: HBM, every row is read once.
-//   k_verify_draw  one cluster of 8 CTAs per request: joins the chunks of each row, walks the drafts, then works on the
+//   k_verify_draw  one cluster of 16 CTAs per request: joins the chunks of each row, walks the drafts, then works on the
 //                  one row that the draw needs. A running sum over 151936 entries that is compared with a border has to
 //                  be the same for whoever forms it, so this row's exponentials and sums are in 64 bits: with 32 the
 //                  drawn index would differ from the exact one about once in 10^4 draws.
@@ -22,6 +22,7 @@
 
 #include "common.cuh"
 #include "kernels.hpp"
+#include "pdl.cuh"
 #include "types16.cuh"
 
 namespace cg = cooperative_groups;
@@ -33,8 +34,8 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowVals = 16;                        // logits a thread holds at a time
 constexpr int kRowTile = kRowThreads * kRowVals;    // 4096
-constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCtas = 8;
-constexpr int kDrawCache = 25600;                   // 64-bit weights a CTA of the draw keeps in shared memory
+constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCtas = 16;
+constexpr int kDrawCache = 12800;                   // 64-bit weights a CTA of the draw keeps in shared memory (two per SM)
 
 struct RowPart {  // of one chunk of a row
   float mx;
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
   const int64_t end = min(begin + static_cast<int64_t>(tiles) * kRowTile, static_cast<int64_t>(a.V));
   // rows whose address is not a multiple of 16 are read value by value
   const bool vec = (reinterpret_cast<uintptr_t>(l) & 15) == 0;
+  pdl_launch();
   float v[kRowVals];
   auto load = [&](int64_t at) {  // tile `at`: W-value words, kRowThreads apart; absent values are -inf
 #pragma unroll
@@ -148,8 +150,8 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
   }
 }
 
-// 2^t for t <= 0 in 64 bits: t = n + f, |f| <= 1/2, the Taylor series of 2^f to degree 11 (remainder
-// (ln 2 / 2)^12 / 12! = 6e-15), n into the exponent. 0 below the normal numbers.
+// 2^t for t <= 0 in 64 bits: t = n + f, |f| <= 1/2, the Taylor series of 2^f to degree 9 (remainder
+// (ln 2 / 2)^10 / 10! = 7e-12), n into the exponent. 0 below the normal numbers.
 __device__ __forceinline__ double exp2_64(double t) {
   if (!(t > -1000.0)) return 0.0;
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it leaves round(t) in the low word
@@ -157,10 +159,8 @@ __device__ __forceinline__ double exp2_64(double t) {
   const double f = t - (m - kRound);
   constexpr double L = 0.693147180559945309417;
   constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
-                   c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
-  double p = c11;
-  p = fma(p, f, c10);
-  p = fma(p, f, c9);
+                   c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9;
+  double p = c9;
   p = fma(p, f, c8);
   p = fma(p, f, c7);
   p = fma(p, f, c6);
@@ -194,15 +194,19 @@ __device__ __forceinline__ void join_row(const RowPart* parts, int n_chunks, dou
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 }
 
+constexpr int kDrawRows = 64;  // rows of a request whose maximum is kept from the walk over its drafts
+
 struct DrawShared {
   int first;                 // first draft that was not kept
+  float mx[kDrawRows];
+  int idx[kDrawRows];
   double warp[kDrawWarps];   // sums of the warps' segments
   double sum[2];             // of this CTA: normalisation, weights
 };
 
 template <typename T>
-__global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads)
-    k_verify_draw(VerifyArgs a, int n_chunks, const RowPart* parts, int cap) {
+__global__ void __launch_bounds__(kDrawThreads, 2)
+    k_verify_draw(VerifyArgs a, int n_chunks, const RowPart* parts, int seg, bool kept) {
   extern __shared__ double cache[];
   __shared__ DrawShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -210,6 +214,8 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = a.row_off[r], hi = a.row_off[r + 1];
   const bool valid = lo >= r && hi > lo && hi <= a.n_rows && hi - 1 - r <= a.n_rows - a.n_req;
+  const float temp = a.temperature[r];
+  pdl_wait();
   if (!valid) {  // the same for all CTAs of the cluster
     if (rank == 0 && tid == 0) {
       a.n_acc[r] = 0;
@@ -219,33 +225,40 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
     return;
   }
   const int k = hi - lo - 1, j0 = lo - r;  // drafts and their first index
-  const float temp = a.temperature[r];
   const bool greedy = !(temp > 0.0f);
   const double c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temp);
   const T* logits = static_cast<const T*>(a.logits);
   if (tid == 0) sh.first = k;
   __syncthreads();
-  for (int i = warp; i < k; i += kDrawWarps) {
+  for (int i = warp; i <= k; i += kDrawWarps) {
+    const int d = i < k ? a.draft[j0 + i] : -1;
+    const bool in = d >= 0 && d < a.V;
+    float l = -INFINITY, qd = 0.0f;
+    if (in && !greedy) {  // issued before the chunks are joined
+      l = to_float(logits[static_cast<int64_t>(lo + i) * a.ld + d]);
+      qd = a.q ? a.q[static_cast<int64_t>(j0 + i) * a.q_ld + d] : 1.0f;
+    }
+    const double ui = a.u[lo + i];
     float mx;
     int idx;
     double sum;
     join_row(parts + static_cast<int64_t>(lo + i) * n_chunks, n_chunks, c, lane, mx, idx, sum);
     if (lane == 0) {
-      const int d = a.draft[j0 + i];
-      const bool in = d >= 0 && d < a.V, some = mx > -INFINITY && mx < INFINITY;
-      double p = 0.0;
-      bool keep;
-      if (greedy) {
-        p = some && d == idx ? 1.0 : 0.0;
-        keep = p > 0.0;
-      } else {
-        const float l = in ? fmaxf(to_float(logits[static_cast<int64_t>(lo + i) * a.ld + d]), -INFINITY) : -INFINITY;
-        if (some) p = exp2_64((static_cast<double>(l) - static_cast<double>(mx)) * c) / sum;
-        const double q = !in ? 0.0 : a.q ? static_cast<double>(a.q[static_cast<int64_t>(j0 + i) * a.q_ld + d]) : 1.0;
-        keep = q > 0.0 && a.u[lo + i] * q < p;
+      if (i < kDrawRows) sh.mx[i] = mx, sh.idx[i] = idx;
+      if (i < k) {
+        const bool some = mx > -INFINITY && mx < INFINITY;
+        double p = 0.0;
+        bool keep;
+        if (greedy) {
+          p = some && d == idx ? 1.0 : 0.0;
+          keep = p > 0.0;
+        } else {
+          if (some) p = exp2_64((static_cast<double>(fmaxf(l, -INFINITY)) - static_cast<double>(mx)) * c) / sum;
+          keep = qd > 0.0f && ui * static_cast<double>(qd) < p;
+        }
+        if (!keep) atomicMin(&sh.first, i);
+        if (rank == 0 && a.p) a.p[j0 + i] = static_cast<float>(p);
       }
-      if (!keep) atomicMin(&sh.first, i);
-      if (rank == 0 && a.p) a.p[j0 + i] = static_cast<float>(p);
     }
   }
   __syncthreads();
@@ -258,8 +271,13 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
   const int row = lo + stop;
   float mx;
   int idx;
-  double unused;
-  join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, lane, mx, idx, unused);
+  if (stop < kDrawRows) {
+    mx = sh.mx[stop];
+    idx = sh.idx[stop];
+  } else {
+    double unused;
+    join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, lane, mx, idx, unused);
+  }
   if (greedy || !(mx > -INFINITY && mx < INFINITY)) {
     if (rank == 0 && tid == 0) a.next[r] = mx > -INFINITY && mx < INFINITY ? idx : -1;
     return;
@@ -269,12 +287,12 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
   const int d = reject ? a.draft[j0 + stop] : -1;
   const float* q = reject && a.q ? a.q + static_cast<int64_t>(j0 + stop) * a.q_ld : nullptr;
   const double u = a.u[row + (reject ? 1 : 0)];
-  // this CTA's slice of the vocabulary, each warp a contiguous segment of it
-  const int slice = (a.V + kDrawCtas - 1) / kDrawCtas, seg = (slice + kDrawWarps - 1) / kDrawWarps;
-  const int s0 = min(a.V, rank * slice), s1 = min(a.V, s0 + slice);
-  const int w0 = min(s1, s0 + warp * seg), w1 = min(s1, w0 + seg);
-  auto weight = [&](int j) {
-    return exp2_64((static_cast<double>(fmaxf(to_float(l[j]), -INFINITY)) - static_cast<double>(mx)) * c);
+  // this CTA's slice of the vocabulary: a contiguous segment of seg values for each warp, a value per lane and step (the
+  // 64-bit weights of a step then lie in consecutive banks; four values a lane took 8 wavefronts a store where this takes 2)
+  const int s0 = rank * kDrawWarps * seg;
+  const int w0 = min(a.V, s0 + warp * seg), w1 = min(a.V, w0 + seg);
+  auto weigh = [&](float x) {
+    return exp2_64((static_cast<double>(fmaxf(x, -INFINITY)) - static_cast<double>(mx)) * c);
   };
   // sums of the CTAs, in rank order
   auto cluster_sum = [&](int which, double v) {
@@ -292,36 +310,64 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
     for (int o = 0; o < kDrawCtas; ++o) t += cluster.map_shared_rank(&sh, o)->sum[which];
     return t;
   };
+  // kU steps' loads are issued before the first is used, those of the draft probabilities before the clusters meet over the
+  // normalisation. The weights stay in shared memory (kept) unless a slice is too long for it; those are formed again.
+  constexpr int kU = 10;
+  float x[kU];
+  auto load = [&](auto* from, int j, float fill) {
+#pragma unroll
+    for (int g = 0; g < kU; ++g) x[g] = j + 32 * g < w1 ? to_float(from[j + 32 * g]) : fill;
+  };
   double v = 0.0;
-#pragma unroll 4
-  for (int j = w0 + lane; j < w1; j += 32) {
-    const double e = weight(j);
-    if (j - s0 < cap) cache[j - s0] = e;
-    v += e;
+  for (int j = w0 + lane; j < w1; j += 32 * kU) {
+    load(l, j, -INFINITY);
+#pragma unroll
+    for (int g = 0; g < kU; ++g) {
+      const double e = weigh(x[g]);  // 0 past the segment
+      if (kept && j + 32 * g < w1) cache[j + 32 * g - s0] = e;
+      v += e;
+    }
   }
+  if (q) load(q, w0 + lane, 0.0f);
   const double Z = cluster_sum(0, v);
   bool residual = reject;
   double total = Z;
-  auto rest = [&](int j, double e) {
-    if (q) return fmax(e - static_cast<double>(q[j]) * Z, 0.0);
+  auto rest = [&](int j, double e, float qj) {
+    if (q) {
+      const double left = e - static_cast<double>(qj) * Z;
+      return left > 0.0 ? left : 0.0;
+    }
     return j == d ? 0.0 : e;  // a draft without probabilities is certain of itself
   };
   if (residual) {
     v = 0.0;
-#pragma unroll 4
-    for (int j = w0 + lane; j < w1; j += 32) {
-      const double e = rest(j, j - s0 < cap ? cache[j - s0] : weight(j));
-      if (j - s0 < cap) cache[j - s0] = e;
-      v += e;
+    if (kept) {
+      for (int j = w0 + lane; j < w1; j += 32 * kU) {
+        if (q && j != w0 + lane) load(q, j, 0.0f);
+#pragma unroll
+        for (int g = 0; g < kU; ++g) {
+          const int at = j + 32 * g;
+          if (at < w1) {
+            const double e = rest(at, cache[at - s0], x[g]);
+            cache[at - s0] = e;
+            v += e;
+          }
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int j = w0 + lane; j < w1; j += 32) v += rest(j, weigh(to_float(l[j])), q ? q[j] : 0.0f);
     }
     total = cluster_sum(1, v);
     if (!(total > 0.0)) {  // p <= q everywhere: draw from p
       residual = false;
       total = Z;
-      for (int j = w0 + lane; j < w1; j += 32)
-        if (j - s0 < cap) cache[j - s0] = weight(j);
       v = 0.0;
-      for (int j = w0 + lane; j < w1; j += 32) v += j - s0 < cap ? cache[j - s0] : weight(j);
+      for (int j = w0 + lane; j < w1; j += 32) {
+        const double e = weigh(to_float(l[j]));
+        if (kept) cache[j - s0] = e;
+        v += e;
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       __syncthreads();
@@ -361,12 +407,14 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
   }
   if (warp != ow) return;
   auto value = [&](int j) {
-    if (j - s0 < cap) return cache[j - s0];
-    return residual ? rest(j, weight(j)) : weight(j);
+    if (kept) return cache[j - s0];
+    const double e = weigh(to_float(l[j]));
+    return residual ? rest(j, e, q ? q[j] : 0.0f) : e;
   };
-  const int part = (w1 - w0 + 31) / 32;
+  const int part = ((w1 - w0 + 31) / 32) | 1;  // odd: the lanes' values lie in different banks
   const int p0 = min(w1, w0 + lane * part), p1 = min(w1, p0 + part);
   double mine = 0.0;
+#pragma unroll 1
   for (int j = p0; j < p1; ++j) mine += value(j);
   double incl = mine;
 #pragma unroll
@@ -377,18 +425,28 @@ __global__ void __cluster_dims__(kDrawCtas, 1, 1) __launch_bounds__(kDrawThreads
   const unsigned reach = __ballot_sync(0xffffffffu, mine > 0.0 && warp_before + incl >= target);
   const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
   const int pick = reach ? __ffs(reach) - 1 : 31 - __clz(some);
-  if (lane != pick) return;
-  double run = warp_before + (incl - mine);
+  // the picked lane's values by the whole warp, 32 at a time, in order
+  const int c0 = __shfl_sync(0xffffffffu, p0, pick), c1 = __shfl_sync(0xffffffffu, p1, pick);
+  double run = warp_before + __shfl_sync(0xffffffffu, incl - mine, pick);
   int found = -1;
-  for (int j = p0; j < p1; ++j) {
-    const double e = value(j);
-    if (e > 0.0) {
-      run += e;
-      found = j;
-      if (run >= target) break;
+  for (int j = c0; j < c1; j += 32) {
+    double e = j + lane < c1 ? value(j + lane) : 0.0;
+    double s = e;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
     }
+    const unsigned pos = __ballot_sync(0xffffffffu, e > 0.0);
+    const unsigned hit = __ballot_sync(0xffffffffu, e > 0.0 && run + s >= target);
+    if (hit) {
+      found = j + __ffs(hit) - 1;
+      break;
+    }
+    if (pos) found = j + 31 - __clz(pos);
+    run += __shfl_sync(0xffffffffu, s, 31);
   }
-  a.next[r] = found;
+  if (lane == 0) a.next[r] = found;
 }
 
 template <typename T>
@@ -399,9 +457,9 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
   RowPart* parts = static_cast<RowPart*>(a.ws);
   k_verify_rows<T><<<dim3(static_cast<unsigned>(a.n_rows), static_cast<unsigned>(n_chunks)), kRowThreads, 0, s>>>(
       a, tiles, n_chunks, parts);
-  const int slice = (a.V + kDrawCtas - 1) / kDrawCtas;
-  const int cap = std::min(slice, kDrawCache);
-  const size_t smem = static_cast<size_t>(cap) * sizeof(double);
+  const int seg = (a.V + kDrawCtas * kDrawWarps * 32 - 1) / (kDrawCtas * kDrawWarps * 32) * 32;
+  const bool kept = seg * kDrawWarps <= kDrawCache;
+  const size_t smem = kept ? static_cast<size_t>(seg) * kDrawWarps * sizeof(double) : 0;
   static bool set[kMaxDevices] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -410,11 +468,14 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
   if (!set[dev]) {
     e = cudaFuncSetAttribute(k_verify_draw<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kDrawCache * static_cast<int>(sizeof(double)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_verify_draw<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     set[dev] = true;
   }
-  k_verify_draw<T><<<static_cast<unsigned>(a.n_req) * kDrawCtas, kDrawThreads, smem, s>>>(a, n_chunks, parts, cap);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_pdl(k_verify_draw<T>, dim3(static_cast<unsigned>(a.n_req) * kDrawCtas), dim3(kDrawThreads), smem, s, kDrawCtas, a,
+                    n_chunks, static_cast<const RowPart*>(parts), seg, kept);
 }
 
 }  // namespace
