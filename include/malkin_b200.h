@@ -414,7 +414,7 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
  * -infinity are tokens that cannot be drawn, NaN logits count as -infinity; a row whose maximum is not finite has no
  * distribution: no draft is kept on it, and as the row drawn from it gives dev_next = -1. A request whose rows are not as
  * above gives dev_n_acc = 0, dev_next = -1 and records MK_ERR_ARG (its dev_p entries are not written).
- * dev_ws: mk_verify_draft_workspace(n_rows, n_req, V) bytes, 16-byte aligned. V at most 2^27. */
+ * dev_ws: mk_verify_draft_workspace(n_rows, n_req, V) bytes, 16-byte aligned. V at most 2^27, n_req at most 65535. */
 int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V);
 int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,
                     const int32_t* dev_row_off, const int32_t* dev_draft, const float* dev_q, int64_t q_ld,

@@ -91,6 +91,7 @@ int current_device() {
 constexpr int kMaxHeads = 1024;
 constexpr int kMaxVocab = 1 << 27;
 constexpr int kMaxReq = 1 << 20;
+constexpr int kMaxVerify = 65535;  // requests of one verification (a grid dimension)
 
 mkb::ActType act_type(int type, bool with_f32, const char* who) {
   if (type == MK_TYPE_F32 && with_f32) return mkb::ActType::f32;
@@ -673,7 +674,7 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
 
 int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V) {
   if (n_rows < 0 || n_req < 0 || V <= 0 || V > kMaxVocab) return -1;
-  return mkb::verify_workspace(n_rows, V);
+  return mkb::verify_workspace(n_rows, n_req, V);
 }
 
 int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,
@@ -685,8 +686,8 @@ int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, in
     const mkb::ActType t = act_type(type, true, who);
     if (n_req < 0 || V <= 0 || V > kMaxVocab || n_rows < n_req) throw mkb::ArgError("verify_draft: bad shape");
     if (ld < V || (dev_q && q_ld < V)) throw mkb::ArgError("verify_draft: rows overlap (a stride is shorter than its row)");
-    if (ws_bytes < mkb::verify_workspace(n_rows, V)) throw mkb::ArgError("verify_draft: workspace too small");
-    if (n_req > kMaxReq) throw mkb::ArgError("verify_draft: too many requests");
+    if (ws_bytes < mkb::verify_workspace(n_rows, n_req, V)) throw mkb::ArgError("verify_draft: workspace too small");
+    if (n_req > kMaxVerify) throw mkb::ArgError("verify_draft: at most 65535 requests");
     if (n_req == 0) return;
     check_dev({{dev_logits, act_size(t), "dev_logits"}, {dev_row_off, 4, "dev_row_off"},
                {dev_draft, 4, "dev_draft", n_rows == n_req}, {dev_q, 4, "dev_q", true},

@@ -286,7 +286,7 @@ struct VerifyArgs {
   int* status;
 };
 // Bytes of VerifyArgs::ws.
-int64_t verify_workspace(int n_rows, int V);
+int64_t verify_workspace(int n_rows, int n_req, int V);
 // 0, or the CUDA error of a launch that could not be queued.
 int launch_verify_draft(const VerifyArgs& a, ActType type, int sms, cudaStream_t s);
 

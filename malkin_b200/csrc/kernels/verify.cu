@@ -8,11 +8,15 @@
 //
 //   k_verify_rows  one CTA per (row, vocabulary chunk): maximum, its lowest index, and sum of exp((l - max) / T).
 //                  Bound: HBM, every row is read once.
-//   k_verify_draw  one cluster of 16 CTAs per request: joins the chunks of each row, walks the drafts, then works on the
-//                  one row that the draw needs. A running sum over 151936 entries that is compared with a border has to
-//                  be the same for whoever forms it, so this row's exponentials and sums are in 64 bits: with 32 the
-//                  drawn index would differ from the exact one about once in 10^4 draws.
-#include <cooperative_groups.h>
+//   k_verify_norm  CTAs (request, chunk): each joins the chunks of the request's rows and walks its drafts (a warp a row;
+//                  cheaper than a kernel of its own), then the chunk's share of the normalisation of the one row that the
+//                  draw needs
+//   k_verify_rest  CTAs (request, chunk): the chunk's share of the draw's total
+//   k_verify_pick  one CTA per request: the chunk, the segment and the token the running sum reaches its target in
+// A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the
+// row's exponentials and sums are in 64 bits: with 32 the drawn index would differ from the exact one about once in 10^4
+// draws. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
+// slower: 93, 85 and 96 us against YY us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -25,17 +29,19 @@
 #include "pdl.cuh"
 #include "types16.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace mkb {
 
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowVals = 16;                        // logits a thread holds at a time
-constexpr int kRowTile = kRowThreads * kRowVals;    // 4096
-constexpr int kDrawThreads = 512, kDrawWarps = kDrawThreads / 32, kDrawCtas = 16;
-constexpr int kDrawCache = 12800;                   // 64-bit weights a CTA of the draw keeps in shared memory (two per SM)
+// A thread holds 64 bytes of a row at a time; a tile is what a block holds.
+template <typename T>
+constexpr int kRowVals = 64 / sizeof(T);
+template <typename T>
+constexpr int kRowTile = kRowThreads * kRowVals<T>;
+constexpr int kDrawThreads = 256, kDrawVals = 16;   // of the normalisation and the rest
+constexpr int kDrawChunk = kDrawThreads * kDrawVals;
+constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 
 struct RowPart {  // of one chunk of a row
   float mx;
@@ -43,9 +49,19 @@ struct RowPart {  // of one chunk of a row
   double sum;
 };
 
-__host__ __device__ inline int verify_chunk_tiles(int n_rows, int V, int sms) {
+struct Decision {  // of a request
+  int32_t draw;    // 1: the token is drawn from `row`; 0: it is written already
+  int32_t row;     // logits row
+  int32_t draft;   // index of the draft refused there, -1: none
+  int32_t token;   // that draft
+  float mx, pad;
+  double c, u;     // log2 e / T, the draw's uniform
+};
+
+template <typename T>
+int verify_chunk_tiles(int n_rows, int V, int sms) {
   // one tile per CTA while that gives fewer than 8 CTAs per SM, else up to four tiles (fewer, longer CTAs)
-  const int64_t tiles = (static_cast<int64_t>(V) + kRowTile - 1) / kRowTile;
+  const int64_t tiles = (static_cast<int64_t>(V) + kRowTile<T> - 1) / kRowTile<T>;
   const int64_t per = tiles * n_rows / (8 * static_cast<int64_t>(sms));
   return static_cast<int>(per < 1 ? 1 : per > 4 ? 4 : per);
 }
@@ -71,20 +87,21 @@ __device__ __forceinline__ void load16b(const T* p, float* v) {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int tiles, int n_chunks, RowPart* parts) {
   constexpr int W = 16 / sizeof(T);  // values per word
+  constexpr int kVals = kRowVals<T>, kTile = kRowTile<T>;
   __shared__ float s_mx[kRowThreads / 32];
   __shared__ int s_idx[kRowThreads / 32];
   __shared__ double s_sum[kRowThreads / 32];
   const int row = blockIdx.x, chunk = blockIdx.y, tid = threadIdx.x;
   const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld;
-  const int64_t begin = static_cast<int64_t>(chunk) * tiles * kRowTile;
-  const int64_t end = min(begin + static_cast<int64_t>(tiles) * kRowTile, static_cast<int64_t>(a.V));
+  const int64_t begin = static_cast<int64_t>(chunk) * tiles * kTile;
+  const int64_t end = min(begin + static_cast<int64_t>(tiles) * kTile, static_cast<int64_t>(a.V));
   // rows whose address is not a multiple of 16 are read value by value
   const bool vec = (reinterpret_cast<uintptr_t>(l) & 15) == 0;
   pdl_launch();
-  float v[kRowVals];
+  float v[kVals];
   auto load = [&](int64_t at) {  // tile `at`: W-value words, kRowThreads apart; absent values are -inf
 #pragma unroll
-    for (int b = 0; b < kRowVals / W; ++b) {
+    for (int b = 0; b < kVals / W; ++b) {
       const int64_t i = at + static_cast<int64_t>(b * kRowThreads + tid) * W;
       if (vec && i + W <= end) {
         load16b<T>(l + i, v + b * W);
@@ -107,7 +124,7 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
   for (int64_t at = begin;;) {
     float m = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kRowVals; ++e) {
+    for (int e = 0; e < kVals; ++e) {
       v[e] = fmaxf(v[e], -INFINITY);  // NaN reads as -inf
       m = fmaxf(m, v[e]);
     }
@@ -115,14 +132,14 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
       sum = mx > -INFINITY ? sum * exp2f((mx - m) * c) : 0.0f;
       mx = m;
 #pragma unroll
-      for (int e = kRowVals - 1; e >= 0; --e)
+      for (int e = kVals - 1; e >= 0; --e)
         if (v[e] == m) idx = static_cast<int>(at + static_cast<int64_t>((e / W) * kRowThreads + tid) * W + e % W);
     }
     if (mx > -INFINITY && sums) {
 #pragma unroll
-      for (int e = 0; e < kRowVals; ++e) sum += exp2f((v[e] - mx) * c);
+      for (int e = 0; e < kVals; ++e) sum += exp2f((v[e] - mx) * c);
     }
-    at += kRowTile;
+    at += kTile;
     if (at >= end) break;
     load(at);
   }
@@ -150,32 +167,37 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
   }
 }
 
-// 2^t for t <= 0 in 64 bits: t = n + f, |f| <= 1/2, the Taylor series of 2^f to degree 9 (remainder
-// (ln 2 / 2)^10 / 10! = 7e-12), n into the exponent. 0 below the normal numbers.
-__device__ __forceinline__ double exp2_64(double t) {
-  if (!(t > -1000.0)) return 0.0;
-  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it leaves round(t) in the low word
+// 2^t for -1000 < t <= 0 in 64 bits: t = n + k / 16 + f with |f| <= 1/32, 2^(k/16) from a table of 16 (one row of shared
+// memory's banks), the Taylor series of 2^f to degree 5 (remainder (ln 2 / 32)^6 / 6! = 1.4e-13), n into the exponent.
+__device__ __forceinline__ double exp2_64(double t, const double* tab) {
+  constexpr double kRound = 6755399441055744.0 / 16;  // 1.5 * 2^48: adding it leaves round(16 t) in the low word
   const double m = t + kRound;
   const double f = t - (m - kRound);
+  const int q = __double2loint(m);
   constexpr double L = 0.693147180559945309417;
-  constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
-                   c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9;
-  double p = c9;
-  p = fma(p, f, c8);
-  p = fma(p, f, c7);
-  p = fma(p, f, c6);
-  p = fma(p, f, c5);
+  constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5;
+  double p = c5;
   p = fma(p, f, c4);
   p = fma(p, f, c3);
   p = fma(p, f, c2);
   p = fma(p, f, c1);
-  p = fma(p, f, 1.0);
-  return __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
+  p = fma(p, f, 1.0) * tab[q & 15];
+  return __hiloint2double(__double2hiint(p) + ((q >> 4) << 20), __double2loint(p));
 }
+// exp((x - mx) / T) in 64 bits with c = log2 e / T: 0 for -infinity, NaN and what is below 2^-1000.
+__device__ __forceinline__ double weigh64(float x, float mx, double c, const double* tab) {
+  const double t = (static_cast<double>(fmaxf(x, -INFINITY)) - static_cast<double>(mx)) * c;
+  return t > -1000.0 ? exp2_64(t, tab) : 0.0;
+}
+__constant__ double kSixteenths[16] = {  // 2^(k/16)
+    1.0, 1.0442737824274138403, 1.0905077326652576592, 1.1387886347566916537, 1.1892071150027210667,
+    1.2418578120734840486, 1.2968395546510096659, 1.3542555469368927283, 1.4142135623730950488, 1.4768261459394993114,
+    1.5422108254079408236, 1.6104903319492543082, 1.6817928305074290861, 1.7562521603732994831, 1.8340080864093424635,
+    1.9152065613971472939};
 
 // Maximum, lowest index and sum of a row from its chunks, by one warp; every lane gets them.
-__device__ __forceinline__ void join_row(const RowPart* parts, int n_chunks, double c, int lane, float& mx, int& idx,
-                                         double& sum) {
+__device__ __forceinline__ void join_row(const RowPart* parts, int n_chunks, double c, const double* tab, int lane,
+                                         float& mx, int& idx, double& sum) {
   mx = -INFINITY;
   idx = INT32_MAX;
   for (int i = lane; i < n_chunks; i += 32)
@@ -188,53 +210,81 @@ __device__ __forceinline__ void join_row(const RowPart* parts, int n_chunks, dou
   }
   sum = 0.0;
   for (int i = lane; i < n_chunks; i += 32)
-    if (parts[i].mx > -INFINITY)
-      sum += parts[i].sum * exp2_64((static_cast<double>(parts[i].mx) - static_cast<double>(mx)) * c);
+    if (parts[i].mx > -INFINITY) sum += parts[i].sum * weigh64(parts[i].mx, mx, c, tab);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 }
 
-constexpr int kDrawRows = 64;  // rows of a request whose maximum is kept from the walk over its drafts
+__device__ __forceinline__ double block_sum(double v, double* part) {  // the same on every thread; part: a value a warp
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0.0;
+  for (unsigned w = 0; w < blockDim.x / 32; ++w) t += part[w];
+  return t;
+}
 
-struct DrawShared {
-  int first;                 // first draft that was not kept
-  float mx[kDrawRows];
-  int idx[kDrawRows];
-  double warp[kDrawWarps];   // sums of the warps' segments
-  double sum[2];             // of this CTA: normalisation, weights
+// Weight of a draw before normalisation: exp((l - mx) / T), and where a draft was refused what is left of it beside the
+// draft's probabilities (Z: the row's sum).
+struct Weigh {
+  float mx, cf;
+  double mx64, c, Z;
+  const double* tab;
+  bool dense;   // a draft with probabilities was refused
+  int token;    // a certain draft that was refused, -1
+  __device__ __forceinline__ Weigh(const Decision& d, const double* t, bool with_q)
+      : mx(d.mx), cf(fminf(static_cast<float>(d.c), FLT_MAX)), mx64(static_cast<double>(d.mx)), c(d.c), Z(0.0), tab(t),
+        dense(d.draft >= 0 && with_q), token(d.draft >= 0 && !with_q ? d.token : -1) {}
+  __device__ __forceinline__ double whole(float x) const {
+    const bool some = (x - mx) * cf > -1000.0f;  // selected, not branched on: the chains of several calls interleave
+    const double y = exp2_64((static_cast<double>(some ? x : mx) - mx64) * c, tab);
+    return some ? y : 0.0;
+  }
+  __device__ __forceinline__ double rest(int j, float x, float q) const {
+    const double e = whole(x);
+    if (!dense) return j == token ? 0.0 : e;
+    const double left = fma(-static_cast<double>(fminf(q, INFINITY)), Z, e);  // a NaN probability leaves nothing
+    return __double2hiint(left) < 0 ? 0.0 : left;
+  }
 };
 
+// Grid: (CTAs of a request, request); each takes `per` of the draw's chunks.
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads, 2)
-    k_verify_draw(VerifyArgs a, int n_chunks, const RowPart* parts, int seg, bool kept) {
-  extern __shared__ double cache[];
-  __shared__ DrawShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int r = blockIdx.x / kDrawCtas, rank = static_cast<int>(cluster.block_rank());
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+__global__ void __launch_bounds__(kDrawThreads) k_verify_norm(VerifyArgs a, int n_chunks, const RowPart* parts,
+                                                              Decision* decide, double* zpart, int chunks, int per) {
+  __shared__ double tab[16], part[kDrawThreads / 32];
+  __shared__ int first;
+  const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = a.row_off[r], hi = a.row_off[r + 1];
   const bool valid = lo >= r && hi > lo && hi <= a.n_rows && hi - 1 - r <= a.n_rows - a.n_req;
   const float temp = a.temperature[r];
-  pdl_wait();
-  if (!valid) {  // the same for all CTAs of the cluster
-    if (rank == 0 && tid == 0) {
+  if (tid < 16) tab[tid] = kSixteenths[tid];
+  const bool writer = blockIdx.x == 0;
+  pdl_launch();
+  if (!valid) {
+    if (writer && tid == 0) {
       a.n_acc[r] = 0;
       a.next[r] = -1;
+      decide[r].draw = 0;
       if (a.status) atomicCAS(a.status, 0, kStatusBadIndex);
     }
+    pdl_wait();
     return;
   }
   const int k = hi - lo - 1, j0 = lo - r;  // drafts and their first index
   const bool greedy = !(temp > 0.0f);
   const double c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temp);
   const T* logits = static_cast<const T*>(a.logits);
-  if (tid == 0) sh.first = k;
+  if (tid == 0) first = k;
   __syncthreads();
-  for (int i = warp; i <= k; i += kDrawWarps) {
-    const int d = i < k ? a.draft[j0 + i] : -1;
+  pdl_wait();
+  for (int i = warp; i < k; i += kDrawThreads / 32) {
+    const int d = a.draft[j0 + i];
     const bool in = d >= 0 && d < a.V;
     float l = -INFINITY, qd = 0.0f;
-    if (in && !greedy) {  // issued before the chunks are joined
+    if (in && !greedy) {
       l = to_float(logits[static_cast<int64_t>(lo + i) * a.ld + d]);
       qd = a.q ? a.q[static_cast<int64_t>(j0 + i) * a.q_ld + d] : 1.0f;
     }
@@ -242,249 +292,253 @@ __global__ void __launch_bounds__(kDrawThreads, 2)
     float mx;
     int idx;
     double sum;
-    join_row(parts + static_cast<int64_t>(lo + i) * n_chunks, n_chunks, c, lane, mx, idx, sum);
+    join_row(parts + static_cast<int64_t>(lo + i) * n_chunks, n_chunks, c, tab, lane, mx, idx, sum);
     if (lane == 0) {
-      if (i < kDrawRows) sh.mx[i] = mx, sh.idx[i] = idx;
-      if (i < k) {
-        const bool some = mx > -INFINITY && mx < INFINITY;
-        double p = 0.0;
-        bool keep;
-        if (greedy) {
-          p = some && d == idx ? 1.0 : 0.0;
-          keep = p > 0.0;
-        } else {
-          if (some) p = exp2_64((static_cast<double>(fmaxf(l, -INFINITY)) - static_cast<double>(mx)) * c) / sum;
-          keep = qd > 0.0f && ui * static_cast<double>(qd) < p;
-        }
-        if (!keep) atomicMin(&sh.first, i);
-        if (rank == 0 && a.p) a.p[j0 + i] = static_cast<float>(p);
+      const bool some = mx > -INFINITY && mx < INFINITY;
+      double p = 0.0;
+      bool keep;
+      if (greedy) {
+        p = some && d == idx ? 1.0 : 0.0;
+        keep = p > 0.0;
+      } else {
+        if (some) p = weigh64(l, mx, c, tab) / sum;
+        keep = qd > 0.0f && ui * static_cast<double>(qd) < p;
       }
+      if (!keep) atomicMin(&first, i);
+      if (writer && a.p) a.p[j0 + i] = static_cast<float>(p);
     }
   }
   __syncthreads();
-  const int stop = sh.first;
-  if (rank == 0) {
+  const int stop = first, row = lo + stop;
+  if (writer) {
     if (a.p)
       for (int i = stop + 1 + tid; i < k; i += kDrawThreads) a.p[j0 + i] = 0.0f;  // never looked at
     if (tid == 0) a.n_acc[r] = stop;
   }
-  const int row = lo + stop;
-  float mx;
+  Decision d;
   int idx;
-  if (stop < kDrawRows) {
-    mx = sh.mx[stop];
-    idx = sh.idx[stop];
-  } else {
-    double unused;
-    join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, lane, mx, idx, unused);
+  double unused;
+  join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, tab, lane, d.mx, idx, unused);
+  const bool some = d.mx > -INFINITY && d.mx < INFINITY;
+  d.draw = some && !greedy;
+  d.row = row;
+  d.draft = stop < k ? j0 + stop : -1;
+  d.token = stop < k ? a.draft[j0 + stop] : -1;
+  d.c = c;
+  d.u = a.u[row + (stop < k ? 1 : 0)];
+  d.pad = 0.0f;
+  if (writer && tid == 0) {
+    decide[r] = d;
+    if (!d.draw) a.next[r] = some ? idx : -1;
   }
-  if (greedy || !(mx > -INFINITY && mx < INFINITY)) {
-    if (rank == 0 && tid == 0) a.next[r] = mx > -INFINITY && mx < INFINITY ? idx : -1;
-    return;
-  }
+  if (!d.draw) return;
   const T* l = logits + static_cast<int64_t>(row) * a.ld;
-  const bool reject = stop < k;
-  const int d = reject ? a.draft[j0 + stop] : -1;
-  const float* q = reject && a.q ? a.q + static_cast<int64_t>(j0 + stop) * a.q_ld : nullptr;
-  const double u = a.u[row + (reject ? 1 : 0)];
-  // this CTA's slice of the vocabulary: a contiguous segment of seg values for each warp, a value per lane and step (the
-  // 64-bit weights of a step then lie in consecutive banks; four values a lane took 8 wavefronts a store where this takes 2)
-  const int s0 = rank * kDrawWarps * seg;
-  const int w0 = min(a.V, s0 + warp * seg), w1 = min(a.V, w0 + seg);
-  auto weigh = [&](float x) {
-    return exp2_64((static_cast<double>(fmaxf(x, -INFINITY)) - static_cast<double>(mx)) * c);
-  };
-  // sums of the CTAs, in rank order
-  auto cluster_sum = [&](int which, double v) {
+  const Weigh w(d, tab, a.q != nullptr);
+  float x[kDrawVals];
+  auto load = [&](int chunk) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) sh.warp[warp] = v;
-    __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int w = 0; w < kDrawWarps; ++w) t += sh.warp[w];
-      sh.sum[which] = t;
+    for (int g = 0; g < kDrawVals; ++g) {
+      const int64_t j = static_cast<int64_t>(chunk) * kDrawChunk + g * kDrawThreads + tid;
+      x[g] = chunk < chunks && j < a.V ? to_float(l[j]) : -INFINITY;
     }
-    cluster.sync();
-    double t = 0.0;
-    for (int o = 0; o < kDrawCtas; ++o) t += cluster.map_shared_rank(&sh, o)->sum[which];
-    return t;
   };
-  // kU steps' loads are issued before the first is used, those of the draft probabilities before the clusters meet over the
-  // normalisation. The weights stay in shared memory (kept) unless a slice is too long for it; those are formed again.
-  constexpr int kU = 10;
-  float x[kU];
-  auto load = [&](auto* from, int j, float fill) {
+  const int c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
+  load(c0);
+  for (int chunk = c0; chunk < c1; ++chunk) {
+    double v = 0.0;
 #pragma unroll
-    for (int g = 0; g < kU; ++g) x[g] = j + 32 * g < w1 ? to_float(from[j + 32 * g]) : fill;
-  };
-  double v = 0.0;
-  for (int j = w0 + lane; j < w1; j += 32 * kU) {
-    load(l, j, -INFINITY);
-#pragma unroll
-    for (int g = 0; g < kU; ++g) {
-      const double e = weigh(x[g]);  // 0 past the segment
-      if (kept && j + 32 * g < w1) cache[j + 32 * g - s0] = e;
-      v += e;
-    }
+    for (int g = 0; g < kDrawVals; ++g) v += w.whole(x[g]);
+    if (chunk + 1 < c1) load(chunk + 1);
+    v = block_sum(v, part);
+    if (tid == 0) zpart[static_cast<int64_t>(r) * chunks + chunk] = v;
   }
-  if (q) load(q, w0 + lane, 0.0f);
-  const double Z = cluster_sum(0, v);
-  bool residual = reject;
-  double total = Z;
-  auto rest = [&](int j, double e, float qj) {
-    if (q) {
-      const double left = e - static_cast<double>(qj) * Z;
-      return left > 0.0 ? left : 0.0;
-    }
-    return j == d ? 0.0 : e;  // a draft without probabilities is certain of itself
-  };
-  if (residual) {
-    v = 0.0;
-    if (kept) {
-      for (int j = w0 + lane; j < w1; j += 32 * kU) {
-        if (q && j != w0 + lane) load(q, j, 0.0f);
-#pragma unroll
-        for (int g = 0; g < kU; ++g) {
-          const int at = j + 32 * g;
-          if (at < w1) {
-            const double e = rest(at, cache[at - s0], x[g]);
-            cache[at - s0] = e;
-            v += e;
-          }
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int j = w0 + lane; j < w1; j += 32) v += rest(j, weigh(to_float(l[j])), q ? q[j] : 0.0f);
-    }
-    total = cluster_sum(1, v);
-    if (!(total > 0.0)) {  // p <= q everywhere: draw from p
-      residual = false;
-      total = Z;
-      v = 0.0;
-      for (int j = w0 + lane; j < w1; j += 32) {
-        const double e = weigh(to_float(l[j]));
-        if (kept) cache[j - s0] = e;
-        v += e;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      __syncthreads();
-      if (lane == 0) sh.warp[warp] = v;
-    }
-  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDrawThreads) k_verify_rest(VerifyArgs a, const Decision* decide, const double* zpart,
+                                                              double* rpart) {
+  __shared__ double tab[16], part[kDrawThreads / 32];
+  const int r = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  if (tid < 16) tab[tid] = kSixteenths[tid];
   __syncthreads();
-  const int which = residual ? 1 : 0;
-  const double target = u * total;
-  // the CTA, the warp, the lane and the entry that the running sum reaches the target in; where rounding leaves a part
-  // short of its own sum, its last entry above 0
-  double before = 0.0;
-  int owner = -1;
-  double owner_before = 0.0;
-  for (int o = 0; o < kDrawCtas; ++o) {
-    const double t = cluster.map_shared_rank(&sh, o)->sum[which];
-    if (t > 0.0) {
-      owner = o;
-      owner_before = before;
-      if (before + t >= target) break;
-    }
-    before += t;
-  }
-  cluster.sync();  // every CTA has read the sums
-  if (owner != rank) return;
-  before = owner_before;
-  int ow = -1;
-  double warp_before = before;
-  for (int w = 0; w < kDrawWarps; ++w) {
-    const double t = sh.warp[w];
-    if (t > 0.0) {
-      ow = w;
-      warp_before = before;
-      if (before + t >= target) break;
-    }
-    before += t;
-  }
-  if (warp != ow) return;
-  auto value = [&](int j) {
-    if (kept) return cache[j - s0];
-    const double e = weigh(to_float(l[j]));
-    return residual ? rest(j, e, q ? q[j] : 0.0f) : e;
-  };
-  const int part = ((w1 - w0 + 31) / 32) | 1;  // odd: the lanes' values lie in different banks
-  const int p0 = min(w1, w0 + lane * part), p1 = min(w1, p0 + part);
-  double mine = 0.0;
-#pragma unroll 1
-  for (int j = p0; j < p1; ++j) mine += value(j);
-  double incl = mine;
+  pdl_launch();
+  pdl_wait();
+  const Decision d = decide[r];
+  if (!d.draw || d.draft < 0) return;  // drawn from p itself: the shares are the normalisation's
+  const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(d.row) * a.ld;
+  const float* q = a.q ? a.q + static_cast<int64_t>(d.draft) * a.q_ld : nullptr;
+  float x[kDrawVals], y[kDrawVals];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+  for (int g = 0; g < kDrawVals; ++g) {
+    const int64_t j = static_cast<int64_t>(chunk) * kDrawChunk + g * kDrawThreads + tid;
+    x[g] = j < a.V ? to_float(l[j]) : -INFINITY;
+    y[g] = q && j < a.V ? q[j] : 0.0f;
   }
-  const unsigned reach = __ballot_sync(0xffffffffu, mine > 0.0 && warp_before + incl >= target);
-  const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-  const int pick = reach ? __ffs(reach) - 1 : 31 - __clz(some);
-  // the picked lane's values by the whole warp, 32 at a time, in order
-  const int c0 = __shfl_sync(0xffffffffu, p0, pick), c1 = __shfl_sync(0xffffffffu, p1, pick);
-  double run = warp_before + __shfl_sync(0xffffffffu, incl - mine, pick);
+  Weigh w(d, tab, q != nullptr);
+  double z = 0.0;
+  for (unsigned i = tid; i < gridDim.x; i += kDrawThreads) z += zpart[static_cast<int64_t>(r) * gridDim.x + i];
+  w.Z = block_sum(z, part);
+  double v = 0.0;
+#pragma unroll
+  for (int g = 0; g < kDrawVals; ++g) v += w.rest(chunk * kDrawChunk + g * kDrawThreads + tid, x[g], y[g]);
+  v = block_sum(v, part);
+  if (tid == 0) rpart[static_cast<int64_t>(r) * gridDim.x + chunk] = v;
+}
+
+// Where a running sum over parts reaches the target: the first part above 0 at or past it, else the last above 0 (where
+// rounding leaves the parts short of their total). One warp; before: the sum ahead of that part.
+__device__ __forceinline__ int reach(const double* p, int n, double target, int lane, double& before) {
+  double run = before;
   int found = -1;
-  for (int j = c0; j < c1; j += 32) {
-    double e = j + lane < c1 ? value(j + lane) : 0.0;
-    double s = e;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const double t = i0 + lane < n ? p[i0 + lane] : 0.0;
+    double s = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += y;
     }
-    const unsigned pos = __ballot_sync(0xffffffffu, e > 0.0);
-    const unsigned hit = __ballot_sync(0xffffffffu, e > 0.0 && run + s >= target);
-    if (hit) {
-      found = j + __ffs(hit) - 1;
-      break;
+    const unsigned some = __ballot_sync(0xffffffffu, t > 0.0);
+    const unsigned hit = __ballot_sync(0xffffffffu, t > 0.0 && run + s >= target);
+    const unsigned at = hit ? hit & (0u - hit) : some ? 0x80000000u >> __clz(some) : 0u;
+    if (at) {
+      const int src = __ffs(at) - 1;
+      found = i0 + src;
+      before = run + __shfl_sync(0xffffffffu, s - t, src);
     }
-    if (pos) found = j + 31 - __clz(pos);
+    if (hit) break;
     run += __shfl_sync(0xffffffffu, s, 31);
   }
-  if (lane == 0) a.next[r] = found;
+  return found;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a, const Decision* decide, const double* zpart,
+                                                              const double* rpart, int chunks) {
+  __shared__ double tab[16], part[2][kPickWarps], seg[kPickWarps];
+  const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid < 16) tab[tid] = kSixteenths[tid];
+  pdl_wait();
+  Decision d = decide[r];
+  if (!d.draw) return;
+  const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(d.row) * a.ld;
+  const double* zp = zpart + static_cast<int64_t>(r) * chunks;
+  const double* rp = rpart + static_cast<int64_t>(r) * chunks;
+  double z = 0.0, t = 0.0;
+  for (int i = tid; i < chunks; i += kPickThreads) {
+    z += zp[i];
+    if (d.draft >= 0) t += rp[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    z += __shfl_xor_sync(0xffffffffu, z, o);
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+  }
+  if (lane == 0) part[0][warp] = z, part[1][warp] = t;
+  __syncthreads();
+  z = t = 0.0;
+  for (int w = 0; w < kPickWarps; ++w) z += part[0][w], t += part[1][w];
+  if (d.draft >= 0 && !(t > 0.0)) d.draft = -1;  // p <= q everywhere: draw from p
+  const float* q = d.draft >= 0 && a.q ? a.q + static_cast<int64_t>(d.draft) * a.q_ld : nullptr;
+  Weigh w(d, tab, q != nullptr);
+  w.Z = z;
+  const double target = d.u * (d.draft >= 0 ? t : z);
+  // every warp finds the chunk; then the chunk's segments, one a warp, the segment's lanes and the lane's values
+  double before = 0.0;
+  const int chunk = reach(d.draft >= 0 ? rp : zp, chunks, target, lane, before);
+  constexpr int kOwn = kDrawChunk / kPickThreads;  // consecutive values of a lane
+  const int64_t j0 = static_cast<int64_t>(max(chunk, 0)) * kDrawChunk + static_cast<int64_t>(tid) * kOwn;
+  float x[kOwn], y[kOwn];
+#pragma unroll
+  for (int g = 0; g < kOwn; ++g) {
+    const bool in = j0 + g < a.V;
+    x[g] = in ? to_float(l[j0 + g]) : -INFINITY;
+    y[g] = in && q ? q[j0 + g] : 0.0f;
+  }
+  double e[kOwn], v = 0.0;
+#pragma unroll
+  for (int g = 0; g < kOwn; ++g) {
+    e[g] = w.rest(static_cast<int>(j0 + g), x[g], y[g]);
+    v += e[g];
+  }
+  double incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double s = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += s;
+  }
+  if (lane == 31) seg[warp] = incl;
+  __syncthreads();
+  if (warp != reach(seg, kPickWarps, target, lane, before)) return;
+  const unsigned some = __ballot_sync(0xffffffffu, v > 0.0);
+  const unsigned hit = __ballot_sync(0xffffffffu, v > 0.0 && before + incl >= target);
+  if (lane != (hit ? __ffs(hit) - 1 : 31 - __clz(some))) return;
+  double run = before + (incl - v);
+  int64_t found = -1;
+#pragma unroll
+  for (int g = 0; g < kOwn; ++g) {
+    if (e[g] > 0.0 && (found < 0 || run < target)) found = j0 + g;
+    run += e[g];
+  }
+  a.next[r] = static_cast<int32_t>(found);
+}
+
+struct VerifyWs {
+  int64_t chunks;  // of the draw
+  int64_t parts, decide, zpart, rpart, bytes;
+};
+VerifyWs verify_ws(int n_rows, int n_req, int V) {
+  VerifyWs w;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t p = at;
+    at = (at + bytes + 255) / 256 * 256;
+    return p;
+  };
+  // chunks of one tile are the most a row can have
+  w.parts = take((static_cast<int64_t>(V) + kRowTile<float> - 1) / kRowTile<float> * n_rows * static_cast<int64_t>(sizeof(RowPart)));
+  w.chunks = (static_cast<int64_t>(V) + kDrawChunk - 1) / kDrawChunk;
+  w.decide = take(n_req * static_cast<int64_t>(sizeof(Decision)));
+  w.zpart = take(n_req * w.chunks * 8);
+  w.rpart = take(n_req * w.chunks * 8);
+  w.bytes = std::max<int64_t>(at, 256);
+  return w;
 }
 
 template <typename T>
 int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
-  const int tiles = verify_chunk_tiles(a.n_rows, a.V, sms);
-  const int n_chunks = static_cast<int>((static_cast<int64_t>(a.V) + static_cast<int64_t>(tiles) * kRowTile - 1) /
-                                        (static_cast<int64_t>(tiles) * kRowTile));
-  RowPart* parts = static_cast<RowPart*>(a.ws);
+  const int tiles = verify_chunk_tiles<T>(a.n_rows, a.V, sms);
+  const int n_chunks = static_cast<int>((static_cast<int64_t>(a.V) + static_cast<int64_t>(tiles) * kRowTile<T> - 1) /
+                                        (static_cast<int64_t>(tiles) * kRowTile<T>));
+  const VerifyWs y = verify_ws(a.n_rows, a.n_req, a.V);
+  uint8_t* p = static_cast<uint8_t*>(a.ws);
+  RowPart* parts = reinterpret_cast<RowPart*>(p + y.parts);
+  Decision* decide = reinterpret_cast<Decision*>(p + y.decide);
+  double* zpart = reinterpret_cast<double*>(p + y.zpart);
+  double* rpart = reinterpret_cast<double*>(p + y.rpart);
   k_verify_rows<T><<<dim3(static_cast<unsigned>(a.n_rows), static_cast<unsigned>(n_chunks)), kRowThreads, 0, s>>>(
       a, tiles, n_chunks, parts);
-  const int seg = (a.V + kDrawCtas * kDrawWarps * 32 - 1) / (kDrawCtas * kDrawWarps * 32) * 32;
-  const bool kept = seg * kDrawWarps <= kDrawCache;
-  const size_t smem = kept ? static_cast<size_t>(seg) * kDrawWarps * sizeof(double) : 0;
-  static bool set[kMaxDevices] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  if (!set[dev]) {
-    e = cudaFuncSetAttribute(k_verify_draw<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kDrawCache * static_cast<int>(sizeof(double)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_verify_draw<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    set[dev] = true;
-  }
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return launch_pdl(k_verify_draw<T>, dim3(static_cast<unsigned>(a.n_req) * kDrawCtas), dim3(kDrawThreads), smem, s, kDrawCtas, a,
-                    n_chunks, static_cast<const RowPart*>(parts), seg, kept);
+  cudaError_t e = cudaGetLastError();
+  const dim3 grid(static_cast<unsigned>(y.chunks), static_cast<unsigned>(a.n_req));
+  // every CTA of a request walks its drafts again, so a request gets no more CTAs than fill the SMs four times over
+  const int most = std::max(1, 4 * sms / a.n_req), per = static_cast<int>((y.chunks + most - 1) / most);
+  const dim3 walk(static_cast<unsigned>((y.chunks + per - 1) / per), static_cast<unsigned>(a.n_req));
+  if (e == cudaSuccess)
+    e = launch_pdl(k_verify_norm<T>, walk, dim3(kDrawThreads), 0, s, 1, a, n_chunks, static_cast<const RowPart*>(parts),
+                   decide, zpart, static_cast<int>(y.chunks), per);
+  if (e == cudaSuccess)
+    e = launch_pdl(k_verify_rest<T>, grid, dim3(kDrawThreads), 0, s, 1, a, static_cast<const Decision*>(decide),
+                   static_cast<const double*>(zpart), rpart);
+  if (e == cudaSuccess)
+    e = launch_pdl(k_verify_pick<T>, dim3(static_cast<unsigned>(a.n_req)), dim3(kPickThreads), 0, s, 1, a,
+                   static_cast<const Decision*>(decide), static_cast<const double*>(zpart),
+                   static_cast<const double*>(rpart), static_cast<int>(y.chunks));
+  return e;
 }
 
 }  // namespace
 
-int64_t verify_workspace(int n_rows, int V) {
-  // chunks of one tile are the most a row can have
-  const int64_t chunks = (static_cast<int64_t>(V) + kRowTile - 1) / kRowTile;
-  return std::max<int64_t>(256, chunks * n_rows * static_cast<int64_t>(sizeof(RowPart)));
-}
+int64_t verify_workspace(int n_rows, int n_req, int V) { return verify_ws(n_rows, n_req, V).bytes; }
 
 int launch_verify_draft(const VerifyArgs& a, ActType type, int sms, cudaStream_t s) {
   if (a.n_req <= 0) return cudaSuccess;
