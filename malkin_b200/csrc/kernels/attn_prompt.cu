@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     float m = -INFINITY, l = 0.0f;                   // maximum in use (of the raw scores), sum of the weights
     bool ok = true;
     for (int j = 0; j < blocks; ++j) {
-      ok = mbar_wait_warp(&sm->s_full[t], j & 1, st, kStatusTimeout);
+      ok = mbar_park_warp(&sm->s_full[t], j & 1, st, kStatusTimeout);
       if (!ok) break;
       tc_fence_after();
       float s[kKeys];
@@ -179,10 +179,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 4; i < kKeys; i += 4) {
+      for (int i = 4; i + 8 <= kKeys; i += 8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[i + e]);
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[kKeys - 4 + e]);
       // scale is positive: the largest score is the largest exponent
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       float scale = 1.0f;
@@ -234,11 +236,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int j = 1; j < nb && ok; ++j) {
       for (int t = 0; t < 2 && ok; ++t) {
         if (j >= (t == 0 ? nb0 : nb1)) continue;
-        ok = mbar_wait_warp(&sm->sc_full[t], (j - 1) & 1, st, kStatusTimeout);
+        ok = mbar_park_warp(&sm->sc_full[t], (j - 1) & 1, st, kStatusTimeout);
         if (!ok) break;
         const float f = sm->scale[t][row];
         if (__any_sync(0xffffffffu, f != 1.0f)) {
-          ok = mbar_wait_warp(&sm->pv_done[t], (j - 1) & 1, st, kStatusTimeout);
+          ok = mbar_park_warp(&sm->pv_done[t], (j - 1) & 1, st, kStatusTimeout);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -260,8 +262,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int t = 0; t < 2 && ok; ++t) {
       const int blocks = t == 0 ? nb0 : nb1;
       if (blocks == 0) continue;
-      ok = mbar_wait_warp(&sm->fin[t], 0, st, kStatusTimeout) &&
-           mbar_wait_warp(&sm->pv_done[t], (blocks - 1) & 1, st, kStatusTimeout);
+      ok = mbar_park_warp(&sm->fin[t], 0, st, kStatusTimeout) &&
+           mbar_park_warp(&sm->pv_done[t], (blocks - 1) & 1, st, kStatusTimeout);
       if (!ok) break;
       tc_fence_after();
       const float inv = 1.0f / sm->sum[t][row];
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // ---------------- MMA ----------------
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t id_s = umma_idesc_16(fmt, false, kRows, kKeys), id_o = umma_idesc_16(fmt, true, kRows, D);
-      auto wait = [&](uint64_t* bar, int parity) { return mbar_wait(bar, parity & 1, st, kStatusTimeout); };
+      auto wait = [&](uint64_t* bar, int parity) { return mbar_park(bar, parity & 1, st, kStatusTimeout); };
       auto scores = [&](int t, int stage) {
         const uint32_t q = smem_addr(smem + S::kQ + t * S::kTile), k = smem_addr(ring(stage));
 #pragma unroll
@@ -360,8 +362,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (!ok && nb > 0) {  // let what was issued end before TMEM and shared memory go
         tc_commit(&sm->pv_done[0]);
-        mbar_wait(&sm->pv_done[0], 0, nullptr, 0);
-        mbar_wait(&sm->pv_done[0], 1, nullptr, 0);
+        mbar_park(&sm->pv_done[0], 0, nullptr, 0);
+        mbar_park(&sm->pv_done[0], 1, nullptr, 0);
       }
     } else if (warp == 13 && lane == 0) {
       // ---------------- loads ----------------
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (nb0) load(&mq, smem + S::kQ, head, lo + q0, &sm->q_full[0]);
       for (int i = 0; i < 2 * nb && ok; ++i) {
         const int s = i % S::kStages, round = i / S::kStages;
-        if (round > 0) ok = mbar_wait(&sm->empty[s], (round - 1) & 1, st, kStatusTimeout);
+        if (round > 0) ok = mbar_park(&sm->empty[s], (round - 1) & 1, st, kStatusTimeout);
         if (!ok) break;
         load(i & 1 ? &mv : &mk, ring(s), kv, lo + (i / 2) * kKeys, &sm->full[s]);
         issued = i + 1;
@@ -384,16 +386,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       // every copy has landed before the block's shared memory goes
       for (int i = max(0, issued - S::kStages); i < issued; ++i)
-        mbar_wait(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout);
-      if (nb0) mbar_wait(&sm->q_full[0], 0, st, kStatusTimeout);
-      if (nb1 && issued) mbar_wait(&sm->q_full[1], 0, st, kStatusTimeout);
+        mbar_park(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout);
+      if (nb0) mbar_park(&sm->q_full[0], 0, st, kStatusTimeout);
+      if (nb1 && issued) mbar_park(&sm->q_full[1], 0, st, kStatusTimeout);
     } else if (warp >= 14 && nb > 0) {
       // ---------------- V tiles whose keys some rows must not see ----------------
       for (int j = nb0 - 1; j < nb; ++j) {
         const int i = 2 * j + 1;
         // the load has been issued, so the stage's phase is this tile's; it is not reused before the tile is checked
-        if (!mbar_wait_warp_sleep(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout, 100) ||
-            !mbar_wait_warp(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout))
+        if (!mbar_park_warp(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout) ||
+            !mbar_park_warp(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout))
           break;
         uint4* v = reinterpret_cast<uint4*>(ring(i % S::kStages));
         bool seen = false;
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int x = (warp - 14) * 32 + lane; x < S::kTile / 16; x += 64) {
           const uint4 q = v[x];
           if (odd16<T>(q.x) || odd16<T>(q.y) || odd16<T>(q.z) || odd16<T>(q.w)) {
-            T e[8];
+            alignas(16) T e[8];
             *reinterpret_cast<uint4*>(e) = q;
 #pragma unroll
             for (int y = 0; y < 8; ++y)

@@ -5,10 +5,11 @@
 // requests, so its K and V are read once for up to 128 rows; the own part once per run of tokens with the same sequence.
 // Softmax parts are joined from (maximum, sum, unnormalised output) triples in fp32.
 //
-//   k_shared_plan     one CTA: tiles of at most 128 rows over (group, prefix) and (run, own rows); the blocks of 64 keys of
+//   k_shared_plan     one CTA: tiles of up to 256 rows over (group, prefix) and (run, own rows); the blocks of 96 keys of
 //                     all (tile, KV head) units form one line that is cut into equal pieces, one per CTA of the next kernel
-//   k_shared_attend   two CTAs per SM, each walks its piece: int8 rows to 16-bit tiles in shared memory, S = Q K^T and
-//                     O += P V on tcgen05, a partial triple per (unit, piece)
+//   k_shared_attend   one CTA per SM walks its piece: int8 rows to fp16 / bf16 tiles in shared memory, S = Q K^T and
+//                     O += P V on tcgen05, a partial triple per (unit, piece). Two streams of 128 rows share each converted
+//                     block where a tile has more than 128 rows; otherwise they take the blocks in turn
 //   k_shared_join     a warp per (token, head): joins its partial triples and the ancestors' few keys
 //
 // int8 values are exact in both 16-bit types. Row scales of K (with scale and log2 e) multiply the scores, those of V the
@@ -23,10 +24,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
 #include "kernels.hpp"
+#include "pdl.cuh"
 #include "tcgen05.cuh"
 #include "types16.cuh"
 
@@ -34,29 +37,31 @@ namespace mkb {
 
 namespace {
 
-constexpr int kTileRows = 128;
-constexpr int kBlock = 64;         // keys
-constexpr int kMinBlocks = 2;      // of a CTA's piece
+constexpr int kTileRows = 128;     // of a stream
+constexpr int kBlock = 96;         // keys: three pairs of K and V tiles and both Q tiles fill the shared memory
+constexpr int kMinPiece = 2;       // places of the line in a CTA's piece; even, see Tile
 constexpr int kPlanThreads = 1024;
-constexpr int kAttendThreads = 384;  // warpgroups: softmax, conversion, MMA (one thread)
-constexpr int kRegsSoftmax = 128, kRegsConvert = 88, kRegsMma = 24;  // sum: 3 x the 80 of the launch
-constexpr int kCtasPerSm = 2;
+constexpr int kAttendThreads = 512;  // warpgroups: softmax of stream 0, of stream 1, conversion, MMA and Q
+constexpr int kRegsSoftmax = 160, kRegsConvert = 104, kRegsMma = 88;  // 2 x 160 + 104 + 88 = 4 x the 128 of the launch
 constexpr float kRaiseMax = 8.0f;   // a row's reference is raised when it is to grow by more (exponents of 2)
 constexpr float kHeadroom = 6.0f;   // of it below the largest weight x scale
 constexpr int kLeastExp = -40;      // of a block's largest V scale: blocks of zeros must not push the sums out of range
 
+// Tokens and keys of a unit (with a KV head). A block takes two places of the line when both streams work on it and one
+// otherwise (rounded up to an even count), so places measure time and an even cut never divides a block.
 struct Tile {
   int32_t t0, nt;      // tokens
   int32_t base, len;   // key rows
-  int32_t blocks;      // of 64 keys
+  int32_t blocks, places;
   int32_t own;         // 1: each token sees its own n_keys of them
-  int64_t first;       // blocks of all KV heads before this tile
+  int32_t dual;        // 1: the streams have different rows
+  int64_t first;       // places of all KV heads before this tile
   int64_t row;         // first partial row
 };
 struct PlanHead {
   int32_t tiles;
-  int32_t per;       // blocks of a piece
-  int64_t total;     // blocks of all units
+  int32_t per;       // places of a piece, even
+  int64_t total;     // places of all units
 };
 
 struct SharedWs {  // the workspace's parts
@@ -71,18 +76,18 @@ struct SharedWs {  // the workspace's parts
   int prefix_tiles;  // room for tiles over prefixes
 };
 
-__host__ __device__ inline int64_t pieces_bound(int blocks, int per) { return (blocks + per - 1) / per + 1; }
+__host__ __device__ inline int64_t pieces_bound(int places, int per) { return (places + per - 1) / per + 1; }
 
 struct WsLayout {
   int64_t prefix_tiles, tiles, rows, head, tile, pre, own, group, ml, o, bytes;
 };
 WsLayout ws_layout(int n, int H, int KV, int D, int n_groups, int ctas) {
-  const int per_tile = kTileRows / (H / KV);  // tokens
+  const int per_tile = 2 * (kTileRows / (H / KV));  // tokens
   WsLayout w;
   w.prefix_tiles = n / per_tile + n_groups;  // a group of x tokens has at most x / per_tile + 1
   w.tiles = w.prefix_tiles + n;
-  // whole pieces (at most one per CTA and one more) of at most 128 rows, and two part pieces per unit and segment
-  w.rows = static_cast<int64_t>(ctas + 1) * kTileRows + 4 * static_cast<int64_t>(n) * H;
+  // whole pieces (at most one per CTA and one more) of at most 256 rows, and two part pieces per unit and segment
+  w.rows = static_cast<int64_t>(ctas + 1) * 2 * kTileRows + 4 * static_cast<int64_t>(n) * H;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t p = at;
@@ -160,10 +165,11 @@ __device__ __forceinline__ int own_keys(const SharedArgs& a, int t, bool* bad) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, SharedWs w, int ctas) {
+  pdl_launch();
   __shared__ int part[33];
   __shared__ int64_t part64[33];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = a.H / a.KV, per_tile = kTileRows / G;
+  const int G = a.H / a.KV, half = kTileRows / G, per_tile = 2 * half;
   bool bad = false;
   for (int t = tid; t < a.n; t += kPlanThreads) w.tok_pre[t] = -1;
   // prefix tiles
@@ -245,8 +251,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
     if (keys > 0) atomicMax(&w.tile[w.tok_own[t]].len, keys);
   }
   __syncthreads();
-  // blocks before each tile, then the pieces' length, then partial rows before each tile
-  int64_t blocks = 0;
+  // places before each tile, then the pieces' length, then partial rows before each tile
+  int64_t places = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int64_t mine = 0;
@@ -254,52 +260,69 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
       Tile& x = w.tile[i];
       if (i >= own0) x.nt = w.tile[i + 1].t0 - x.t0;
       x.blocks = (x.len + kBlock - 1) / kBlock;
-      mine = static_cast<int64_t>(x.blocks) * a.KV;
+      x.dual = x.nt > half;
+      x.places = x.dual ? 2 * x.blocks : (x.blocks + 1) / 2 * 2;
+      mine = static_cast<int64_t>(x.places) * a.KV;
     }
     int64_t total;
     const int64_t incl = block_scan_sum(mine, part64, total);
-    if (i < n_tiles) w.tile[i].first = blocks + incl - mine;
-    blocks += total;
+    if (i < n_tiles) w.tile[i].first = places + incl - mine;
+    places += total;
   }
-  const int per = static_cast<int>(max(static_cast<int64_t>(kMinBlocks), (blocks + ctas - 1) / ctas));
+  const int per = static_cast<int>(max(static_cast<int64_t>(kMinPiece), (places + 2 * ctas - 1) / (2 * ctas) * 2));
   int64_t rows = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int64_t mine = 0;
     if (i < n_tiles && w.tile[i].blocks > 0)
-      mine = pieces_bound(w.tile[i].blocks, per) * a.KV * w.tile[i].nt * G;
+      mine = pieces_bound(w.tile[i].places, per) * a.KV * w.tile[i].nt * G;
     int64_t total;
     const int64_t incl = block_scan_sum(mine, part64, total);
     if (i < n_tiles) w.tile[i].row = rows + incl - mine;
     rows += total;
   }
-  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows ? blocks : 0};
+  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows ? places : 0};
   if (bad && a.status) atomicCAS(a.status, 0, kStatusBadIndex);
 }
 
-// ---------------- walk over a CTA's piece ----------------
-struct Walk {
-  int64_t at, end;  // blocks of the line
-  int tile, kv, per;
-  Tile x;
-  // the current part: blocks b0 .. b1 - 1 of (tile, kv), its partial rows from `row`
-  int b0, b1;
-  int64_t row;
+// ---------------- a CTA's piece of the line, part by part ----------------
+// One (tile, KV head) unit's share of the piece. One warp walks the plan and hands the parts to the others through a ring in
+// shared memory, so that nobody else keeps the walk's state in registers.
+struct Part {
+  int b0, nb;      // blocks; nb 0: the piece has ended
+  int t0, nt;      // tokens
+  int len, kv;
+  bool own, dual;
+  int64_t key0;    // the first key's row in the cache planes
+  int64_t row;     // first partial row
+};
 
-  __device__ __forceinline__ void part(const SharedArgs& a, int G) {
-    const int64_t first = x.first + static_cast<int64_t>(kv) * x.blocks;
-    b0 = static_cast<int>(at - first);
-    b1 = static_cast<int>(min(static_cast<int64_t>(x.blocks), static_cast<int64_t>(b0) + (end - at)));
-    const int64_t p = at / per - first / per;
-    row = x.row + (kv * pieces_bound(x.blocks, per) + p) * x.nt * G;
+struct Walk {
+  int done, tile, kv, span;  // places before the current part, its unit and its places
+
+  // The part that begins at `done` (nb 0: none).
+  __device__ __forceinline__ Part part(const SharedArgs& a, const SharedWs& w, int cta, int G) {
+    Part p{};
+    const PlanHead h = *w.head;
+    const int64_t from = static_cast<int64_t>(cta) * h.per, at = from + done, end = min(h.total, from + h.per);
+    if (at >= end || tile >= h.tiles) return p;
+    const Tile x = w.tile[tile];
+    const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
+    const int p0 = static_cast<int>(at - first);
+    const int p1 = static_cast<int>(min(static_cast<int64_t>(x.places), p0 + (end - at)));
+    span = p1 - p0;
+    p.b0 = x.dual ? p0 / 2 : p0;
+    p.nb = (x.dual ? p1 / 2 : min(p1, x.blocks)) - p.b0;
+    p.t0 = x.t0, p.nt = x.nt, p.len = x.len, p.kv = kv;
+    p.own = x.own != 0, p.dual = x.dual != 0;
+    p.key0 = static_cast<int64_t>(kv) * a.n_rows + x.base;
+    p.row = x.row + (kv * pieces_bound(x.places, h.per) + (at / h.per - first / h.per)) * x.nt * G;
+    return p;
   }
   // One whole warp calls it.
-  __device__ __forceinline__ bool begin(const SharedArgs& a, const SharedWs& w, int cta, int G, int lane) {
+  __device__ __forceinline__ Part begin(const SharedArgs& a, const SharedWs& w, int cta, int G, int lane) {
     const PlanHead h = *w.head;
-    per = h.per;
-    at = static_cast<int64_t>(cta) * per;
-    end = min(h.total, at + per);
-    if (at >= end) return false;
+    const int64_t at = static_cast<int64_t>(cta) * h.per;
     // the last tile that begins at or before `at`: 32 probes a round
     int lo = 0, hi = h.tiles;
     while (hi - lo > 1) {
@@ -310,22 +333,20 @@ struct Walk {
       lo = lo + k * step;
       hi = min(hi, lo + step);
     }
+    done = 0;
     tile = lo;
-    x = w.tile[tile];
-    kv = static_cast<int>((at - x.first) / x.blocks);
-    part(a, G);
-    return true;
+    kv = static_cast<int>((at - w.tile[lo].first) / w.tile[lo].places);
+    return part(a, w, cta, G);
   }
-  __device__ __forceinline__ bool next(const SharedArgs& a, const SharedWs& w, int G) {
-    at += b1 - b0;
-    if (at >= end) return false;
+  __device__ __forceinline__ Part next(const SharedArgs& a, const SharedWs& w, int cta, int G) {
+    done += span;
     if (++kv == a.KV) {
       kv = 0;
-      do x = w.tile[++tile];
-      while (x.blocks == 0);
+      ++tile;
+      const int tiles = w.head->tiles;
+      while (tile < tiles && w.tile[tile].blocks == 0) ++tile;
     }
-    part(a, G);
-    return true;
+    return part(a, w, cta, G);
   }
 };
 
@@ -362,101 +383,133 @@ __device__ __forceinline__ uint2 widen4<__nv_bfloat16>(uint32_t w) {
 template <int D>
 struct SharedShape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kQHalf = kTileRows * 128;      // bytes of 64 columns of the Q tile
-  static constexpr int kKvHalf = kBlock * 128;        // of a K or V tile
+  static constexpr int kQHalf = kTileRows * 128;  // bytes of 64 columns of a Q tile
+  static constexpr int kKvHalf = kBlock * 128;    // of a K or V tile
   static constexpr int kQ = kHalves * kQHalf, kKv = kHalves * kKvHalf;
-  static constexpr int kStages = 2;
-  static constexpr int kRing = kQ, kSmall = kQ + kStages * 2 * kKv;
-  static constexpr int kTmem = 256;  // columns: S | S | O
+  static constexpr int kRing = 2 * kQ, kSlots = 6, kSmall = kRing + kSlots * kKv;
 };
+constexpr int kScaleSlots = 4;  // a block's scales are overwritten four blocks later, after its P V (the ring holds three)
+constexpr int kAhead = 1;       // blocks whose rows are in flight in the conversion warps' registers
+constexpr int kParts = 4;       // parts known ahead
 struct SharedSmall {
-  uint64_t q_full, q_empty, full[2], empty[2], s_full[2], p_full[2], pv_done, o_free;
-  float ks[2][kBlock];  // K scale x scale x log2 e
-  float vs[2][kBlock];
-  float vmax[2][2];         // largest finite |V scale| of each half of the block
+  uint64_t part_full[kParts], part_empty[kParts];
+  uint64_t q_full, q_empty, full[6], empty[6], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
+  alignas(16) float ks[kScaleSlots][kBlock];  // K scale x scale x log2 e
+  alignas(16) float vs[kScaleSlots][kBlock];
+  alignas(16) float vmax[kScaleSlots][4];     // largest finite |V scale| of each 32 keys of the block
+  Part part[kParts];
+  float2 ml[kTileRows];           // stream 1's reference and sum, for stream 0 where they share the rows
   uint32_t tmem;
 };
+static_assert(offsetof(SharedSmall, ks) % 16 == 0 && offsetof(SharedSmall, vs) % 16 == 0 &&
+                  offsetof(SharedSmall, vmax) % 16 == 0 && sizeof(float) * kBlock % 16 == 0,
+              "scales are read as 16-byte words");
 template <int D>
 constexpr int shared_smem() {
+  static_assert(SharedShape<D>::kSmall % 1024 == 0, "tiles of whole swizzle atoms");
   return SharedShape<D>::kSmall + static_cast<int>(sizeof(SharedSmall));
 }
+constexpr uint32_t kTmemS = 128, kTmemO = 256;  // columns: S0 | S1 at 0 and 128, O0 | O1 from 256
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(SharedArgs a, SharedWs w) {
+__global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs a, SharedWs w) {
   using S = SharedShape<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   SharedSmall* sm = reinterpret_cast<SharedSmall*>(smem + S::kSmall);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.H / a.KV;
-  Walk walk;
-  if (!walk.begin(a, w, blockIdx.x, G, lane)) return;  // the same for every warp of the block
-  if (warp == 8) tmem_alloc(&sm->tmem, S::kTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.H / a.KV, half = kTileRows / G;
+  pdl_launch();
+  pdl_wait();
+  {
+    const PlanHead h = *w.head;
+    if (static_cast<int64_t>(blockIdx.x) * h.per >= h.total) return;
+  }
+  if (warp == 12) tmem_alloc(&sm->tmem, 512);
   if (threadIdx.x == 0) {
-    mbar_init(&sm->q_full, 128);
+    mbar_init(&sm->q_full, 64);
+    for (int i = 0; i < kParts; ++i) {
+      mbar_init(&sm->part_full[i], 1);
+      mbar_init(&sm->part_empty[i], 15);  // 8 softmax, 4 conversion and 2 Q warps, the MMA thread
+    }
     mbar_init(&sm->q_empty, 1);
-    mbar_init(&sm->pv_done, 1);
-    mbar_init(&sm->o_free, 4);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(&sm->b_fin, 4);
+    for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(&sm->full[i], 128);
       mbar_init(&sm->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sm->s_full[i], 1);
       mbar_init(&sm->p_full[i], 4);
+      mbar_init(&sm->pv_done[i], 1);
+      mbar_init(&sm->o_free[i], 4);
     }
     mbar_fence_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm->tmem, tmem_o = tmem + 2 * kBlock;
+  const uint32_t tmem = sm->tmem;
   int* const st = a.status;
-  auto k_tile = [&](int s) { return smem + S::kRing + s * 2 * S::kKv; };
-  auto v_tile = [&](int s) { return smem + S::kRing + s * 2 * S::kKv + S::kKv; };
+  // part i of the piece, once it is known; nb 0 (or a wait that ran out: ok false) ends the role's loop
+  auto take = [&](uint32_t i, bool& ok) -> const Part& {
+    ok = mbar_park_warp(&sm->part_full[i % kParts], (i / kParts) & 1, st, kStatusTimeout);
+    return sm->part[i % kParts];
+  };
+  auto give_back = [&](uint32_t i) { mbar_arrive(&sm->part_empty[i % kParts]); };
+  auto slot = [&](uint32_t i) { return smem + S::kRing + (i % S::kSlots) * S::kKv; };
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---------------- softmax, rescaling, partial results ----------------
     regs_up<kRegsSoftmax>();
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    uint32_t gb = 0;  // blocks of this CTA so far
+    const int s = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + s * kTmemS + lanes, to = tmem + kTmemO + s * D + lanes;
+    uint32_t gb = 0;              // blocks of this CTA before the part
+    uint32_t mine = 0, other = 0; // blocks of this stream and of the other one so far
+    uint32_t splits = 0;          // parts whose rows the streams shared
     bool ok = true;
-    do {
-      const int rows = walk.x.nt * G;
-      const bool on = warp * 32 < rows;
+    for (uint32_t part = 0;; ++part) {
+      const Part& pt = take(part, ok);
+      if (!ok || pt.nb == 0) break;
+      const bool dual = pt.dual;
+      const int rows = (dual ? (s ? pt.nt - half : half) : pt.nt) * G;
+      const bool on = (warp & 3) * 32 < rows;
       int limit = 0;  // keys this row sees
-      if (row < rows) limit = walk.x.own ? own_keys(a, walk.x.t0 + row / G, nullptr) : walk.x.len;
+      if (row < rows) limit = pt.own ? own_keys(a, pt.t0 + (dual && s ? half : 0) + row / G, nullptr) : pt.len;
+      limit -= pt.b0 * kBlock;
       float m = -INFINITY, l = 0.0f;
-      for (int b = walk.b0; b < walk.b1 && ok; ++b, ++gb) {
-        const int s = gb & 1;
-        ok = mbar_wait_warp(&sm->s_full[s], (gb >> 1) & 1, st, kStatusTimeout);
+      const int nb = pt.nb, step = dual ? 1 : 2, j0 = dual ? 0 : s;
+      for (int j = j0; j < nb; j += step, ++mine) {
+        const int sl = (gb + j) & (kScaleSlots - 1);
+        ok = mbar_park_warp(&sm->s_full[s], mine & 1, st, kStatusTimeout);
         if (!ok) break;
         if (on) {
           tc_fence_after();
-          const uint32_t ts = tmem + s * kBlock + lanes;
           float x[kBlock];
-          tmem_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(x));
-          tmem_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+#pragma unroll
+          for (int c = 0; c < kBlock / 32; ++c) tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
           tmem_wait_ld();
-          const float4* ks = reinterpret_cast<const float4*>(sm->ks[s]);
-          const float4* vs = reinterpret_cast<const float4*>(sm->vs[s]);
+          const float4* ks = reinterpret_cast<const float4*>(sm->ks[sl]);
+          const float4* vs = reinterpret_cast<const float4*>(sm->vs[sl]);
+          const int left = limit - j * kBlock;
+          const bool cut = __any_sync(0xffffffffu, left < kBlock);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int i = 0; i < kBlock / 4; ++i) {
             const float4 k4 = ks[i];
-            x[4 * i] *= k4.x, x[4 * i + 1] *= k4.y, x[4 * i + 2] *= k4.z, x[4 * i + 3] *= k4.w;
-          }
-          const int left = limit - b * kBlock;
-          const bool cut = __any_sync(0xffffffffu, left < kBlock);
-          if (cut) {
+            const f2 y0 = f2_mul(f2_make(x[4 * i], x[4 * i + 1]), f2_make(k4.x, k4.y));
+            const f2 y1 = f2_mul(f2_make(x[4 * i + 2], x[4 * i + 3]), f2_make(k4.z, k4.w));
+            x[4 * i] = f2_lo(y0), x[4 * i + 1] = f2_hi(y0), x[4 * i + 2] = f2_lo(y1), x[4 * i + 3] = f2_hi(y1);
+            if (cut) {  // a masked key's scales may be anything
 #pragma unroll
-            for (int i = 0; i < kBlock; ++i)
-              if (i >= left) x[i] = -INFINITY;
-          }
-          float mx[4] = {x[0], x[1], x[2], x[3]};
+              for (int e = 0; e < 4; ++e)
+                if (4 * i + e >= left) x[4 * i + e] = -INFINITY;
+            }
 #pragma unroll
-          for (int i = 4; i < kBlock; i += 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[4 * i + e]);
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const float big = fmaxf(sm->vmax[s][0], sm->vmax[s][1]);
+          const float4 vm = *reinterpret_cast<const float4*>(sm->vmax[sl]);
+          const float big = fmaxf(fmaxf(vm.x, vm.y), vm.z);
           const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, kLeastExp);
           const float want = top + (static_cast<float>(e) - kHeadroom);
           float scale = 1.0f;
@@ -464,38 +517,38 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
             scale = ex2_approx(m - want);
             m = want;
           }
-          if (b > walk.b0 && __any_sync(0xffffffffu, scale != 1.0f)) {
-            ok = mbar_wait_warp(&sm->pv_done, (gb - 1) & 1, st, kStatusTimeout);
+          if (j > j0 && __any_sync(0xffffffffu, scale != 1.0f)) {
+            ok = mbar_park_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t v[32];
-              tmem_ld32(tmem_o + 32 * c + lanes, v);
+              tmem_ld32(to + 32 * c, v);
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * scale);
-              tmem_st32(tmem_o + 32 * c + lanes, v);
+              tmem_st32(to + 32 * c, v);
             }
           }
           const float ref = m == -INFINITY ? 0.0f : m;
           const f2 m2 = f2_make(-ref, -ref);
           f2 sum2 = f2_make(0.0f, 0.0f);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < kBlock / 32; ++c) {
             uint32_t p[16];
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const float4 v4 = vs[8 * c + i / 2];
-              const int j = 32 * c + 2 * i;
-              const f2 y0 = f2_add(f2_make(x[j], x[j + 1]), m2), y1 = f2_add(f2_make(x[j + 2], x[j + 3]), m2);
+              const int k = 32 * c + 2 * i;
+              const f2 y0 = f2_add(f2_make(x[k], x[k + 1]), m2), y1 = f2_add(f2_make(x[k + 2], x[k + 3]), m2);
               const f2 e0 = f2_make(ex2_approx(f2_lo(y0)), ex2_approx(f2_hi(y0)));
               const f2 e1 = f2_make(ex2_approx(f2_lo(y1)), ex2_approx(f2_hi(y1)));
               sum2 = f2_add(sum2, f2_add(e0, e1));
               f2 w0 = f2_mul(e0, f2_make(v4.x, v4.y)), w1 = f2_mul(e1, f2_make(v4.z, v4.w));
-              if (cut) {  // a masked key's scale may be anything
-                w0 = f2_make(j < left ? f2_lo(w0) : 0.0f, j + 1 < left ? f2_hi(w0) : 0.0f);
-                w1 = f2_make(j + 2 < left ? f2_lo(w1) : 0.0f, j + 3 < left ? f2_hi(w1) : 0.0f);
+              if (cut) {
+                w0 = f2_make(k < left ? f2_lo(w0) : 0.0f, k + 1 < left ? f2_hi(w0) : 0.0f);
+                w1 = f2_make(k + 2 < left ? f2_lo(w1) : 0.0f, k + 3 < left ? f2_hi(w1) : 0.0f);
               }
               p[i] = pack2<__half>(f2_lo(w0), f2_hi(w0));
               p[i + 1] = pack2<__half>(f2_lo(w1), f2_hi(w1));
@@ -510,174 +563,312 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
         if (lane == 0) mbar_arrive(&sm->p_full[s]);
       }
       if (!ok) break;
-      ok = mbar_wait_warp(&sm->pv_done, (gb - 1) & 1, st, kStatusTimeout);
+      const int n_mine = dual ? nb : (nb + 1 - s) / 2, n_other = dual ? nb : nb - n_mine;
+      other += n_other;
+      if (n_mine > 0) ok = mbar_park_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
       if (!ok) break;
-      if (on) {
-        tc_fence_after();
-        if (row < rows) w.ml[walk.row + row] = make_float2(m, l);
-        float* o = w.o + (walk.row + row) * D;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld32(tmem_o + 32 * c + lanes, v);
-          tmem_wait_ld();
-          if (row < rows) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(o + 32 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
-          __syncwarp();
-        }
+      tc_fence_after();
+      if (!dual && s == 1) {
+        // stream 0 has taken the last part's: with no block in this part, nothing else holds this stream back
+        if (part > 0) ok = mbar_park_warp(&sm->o_free[1], (part - 1) & 1, st, kStatusTimeout);
+        if (!ok) break;
+        sm->ml[row] = make_float2(m, l);
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm->b_fin);
+      } else {
+        float f0 = 1.0f, f1 = 0.0f;
+        const bool join = !dual && n_other > 0;
+        if (!dual) {
+          ok = mbar_park_warp(&sm->b_fin, splits & 1, st, kStatusTimeout) &&
+               (n_other == 0 || mbar_park_warp(&sm->pv_done[1], (other - 1) & 1, st, kStatusTimeout));
+          if (!ok) break;
+          tc_fence_after();
+          const float2 o = sm->ml[row];
+          if (join && !(o.x == -INFINITY && o.y == 0.0f)) {
+            const float top = fmaxf(m, o.x);
+            f0 = m == -INFINITY ? 0.0f : ex2_approx(m - top);
+            f1 = ex2_approx(o.x - top);
+            m = top;
+            l = l * f0 + o.y * f1;
+          }
+        }
+        if (on) {
+          const int64_t r = pt.row + (dual && s ? half * G : 0) + row;
+          if (row < rows) w.ml[r] = make_float2(m, l);
+          float* o = w.o + r * D;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld32(to + 32 * c, v);
+            tmem_wait_ld();
+            if (join) {
+              uint32_t u[32];
+              tmem_ld32(to + D + 32 * c, u);
+              tmem_wait_ld();
+              // a row that sees none of a stream's keys has weights 0 there, and an output of 0
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                v[i] = __float_as_uint(__uint_as_float(v[i]) * f0 + __uint_as_float(u[i]) * f1);
+            }
+            if (row < rows) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(o + 32 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
+            __syncwarp();
+          }
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm->o_free[s]);
+          if (!dual) mbar_arrive(&sm->o_free[1]);
+        }
       }
+      if (!dual) ++splits;
+      gb += nb;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->o_free);
-    } while (walk.next(a, w, G));
-  } else if (warp < 8) {
-    // ---------------- Q, and the cache rows as 16-bit tiles ----------------
-    // thread: 16 int8 values (one load) at column block c4 of rows r, r + 32, in both halves of 64 columns. The eight
-    // threads of a store phase hold two rows x four blocks, which the swizzle spreads over all banks.
-    regs_up<kRegsConvert>();
-    const int t = threadIdx.x - 128, c4 = t & 3, r0 = t >> 2;
-    constexpr int L = 2 * S::kHalves;  // loads of each of K and V
+      if (lane == 0) give_back(part);
+    }
+  } else if (warp < 12) {
+    // ---------------- cache rows as 16-bit tiles ----------------
+    // thread: 16 int8 values (one load) at column block c4 of rows r, r + 32, r + 64, in each half of 64 columns. The eight
+    // threads of a store phase hold two rows x four blocks, which the swizzle spreads over all banks. The rows of the next
+    // block are in flight in registers.
+    regs_down<kRegsConvert>();
+    const int t = threadIdx.x - 256, c4 = t & 3, r0 = t >> 2;
+    constexpr int L = 3 * S::kHalves;  // loads of each of K and V
     const float kscale = a.scale * 1.44269504088896341f;
-    uint4 kreg[L], vreg[L];
-    float sreg = 0.0f;
-    uint32_t gb = 0, part = 0;
+    struct Rows {
+      uint4 k[L], v[L];
+      float ks, vs;
+    } regs[kAhead];
+    uint32_t gb = 0;
     bool ok = true;
-    // key rows of a part: the first one's index in the cache planes, and how many there are
-    auto first_row = [&]() { return static_cast<int64_t>(walk.kv) * a.n_rows + walk.x.base; };
-    auto load_row = [&](const int8_t* p, int64_t row0, int len, int b, int i) {
-      const int key = b * kBlock + r0 + 32 * (i & 1);
-      if (key >= len) return make_uint4(0, 0, 0, 0);
-      return ld_stream16(p + (row0 + key) * D + 64 * (i >> 1) + 16 * c4);
+    // the block whose rows are loaded next
+    uint32_t part = 0;
+    int64_t row0 = 0;
+    int len = 0, b = 0, end = 0, ahead = 0;  // ahead: blocks loaded and not yet stored
+    bool more = true;
+    auto open = [&]() {
+      const Part& pt = take(part, ok);
+      more = ok && pt.nb > 0;
+      row0 = pt.key0;
+      len = pt.len;
+      b = pt.b0;
+      end = pt.b0 + pt.nb;
+      __syncwarp();
+      if (more && lane == 0) give_back(part);
+      ++part;
     };
-    auto load_scale = [&](int64_t row0, int len, int b) {  // threads 0..63: K, 64..127: V
-      const int key = b * kBlock + (t & 63);
-      if (key >= len) return 0.0f;
-      return t < 64 ? a.ks[row0 + key] * kscale : a.vs[row0 + key];
+    auto load_row = [&](const int8_t* p, int i) {
+      const int key = b * kBlock + r0 + 32 * (i % 3);
+      if (!more || key >= len) return make_uint4(0, 0, 0, 0);
+      return ld_stream16(p + (row0 + key) * D + 64 * (i / 3) + 16 * c4);
+    };
+    auto load_scales = [&](Rows& r) {
+      const int key = b * kBlock + t;
+      const bool in = more && t < kBlock && key < len;
+      r.ks = in ? a.ks[row0 + key] * kscale : 0.0f;
+      r.vs = in ? a.vs[row0 + key] : 0.0f;
+    };
+    auto advance = [&]() {
+      if (!more) return;
+      ++ahead;
+      if (++b == end) open();
     };
     auto store_row = [&](uint8_t* tile, int i, uint4 v, auto tag) {
       using E = decltype(tag);
-      const int r = r0 + 32 * (i & 1);
-      uint8_t* base = tile + (i >> 1) * S::kKvHalf + r * 128;
+      const int r = r0 + 32 * (i % 3);
+      uint8_t* base = tile + (i / 3) * S::kKvHalf + r * 128;
       const uint2 a0 = widen4<E>(v.x), a1 = widen4<E>(v.y), a2 = widen4<E>(v.z), a3 = widen4<E>(v.w);
       *reinterpret_cast<uint4*>(base + (((2 * c4) ^ (r & 7)) * 16)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
       *reinterpret_cast<uint4*>(base + (((2 * c4 + 1) ^ (r & 7)) * 16)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
     };
-    int64_t row0 = first_row();
-    int len = walk.x.len;
+    auto convert = [&](Rows& r) {  // stores block gb, then loads the one kAhead blocks later into the same registers
+      const int sl = gb & (kScaleSlots - 1);
+      const uint32_t ki = 2 * gb, vi = 2 * gb + 1;
+      if (ki >= S::kSlots) ok = mbar_park_warp(&sm->empty[ki % S::kSlots], (ki / S::kSlots - 1) & 1, st, kStatusTimeout);
+      if (!ok) return;
+      if (t < kBlock) {
+        sm->ks[sl][t] = r.ks;
+        sm->vs[sl][t] = r.vs;
+        const float big = warp_max(fabsf(r.vs) < INFINITY ? fabsf(r.vs) : 0.0f);
+        if (lane == 0) sm->vmax[sl][t >> 5] = big;
+      }
+      load_scales(r);
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      kreg[i] = load_row(a.k, row0, len, walk.b0, i);
-      vreg[i] = load_row(a.v, row0, len, walk.b0, i);
-    }
-    sreg = load_scale(row0, len, walk.b0);
-    bool more = true;
-    while (more && ok) {
-      // Q of this part: 128 rows, those without a token are 0
-      if (part > 0) ok = mbar_wait_warp(&sm->q_empty, (part - 1) & 1, st, kStatusTimeout);
-      if (!ok) break;
-      const int rows = walk.x.nt * G;
-#pragma unroll 4
-      for (int i = t; i < kTileRows * (D / 8); i += 128) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows)
-          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<int64_t>(walk.x.t0 + r / G) * a.q_ld +
-                                              static_cast<int64_t>(walk.kv * G + r % G) * D + 8 * c);
-        *reinterpret_cast<uint4*>(smem + (c / 8) * S::kQHalf + r * 128 + (((c % 8) ^ (r & 7)) * 16)) = v;
+      for (int i = 0; i < L; ++i) {
+        store_row(slot(ki), i, r.k[i], T());
+        r.k[i] = load_row(a.k, i);
       }
       fence_async_smem();
-      mbar_arrive(&sm->q_full);
-      ++part;
-      const int b0 = walk.b0, b1 = walk.b1;
-      more = walk.next(a, w, G);
-      for (int b = b0; b < b1 && ok; ++b, ++gb) {
-        const int s = gb & 1;
-        if (gb >= 2) ok = mbar_wait_warp(&sm->empty[s], ((gb >> 1) - 1) & 1, st, kStatusTimeout);
-        if (!ok) break;
-        int nb = b + 1;  // the next block, whose rows are loaded while this one is stored
-        if (nb == b1) {
-          nb = walk.b0;
-          row0 = first_row();
-          len = more ? walk.x.len : 0;
-        }
-        (t < 64 ? sm->ks[s] : sm->vs[s])[t & 63] = sreg;
-        if (t >= 64) {
-          const float big = warp_max(fabsf(sreg) < INFINITY ? fabsf(sreg) : 0.0f);
-          if (lane == 0) sm->vmax[s][(t - 64) >> 5] = big;
-        }
+      mbar_arrive(&sm->full[ki % S::kSlots]);
+      if (vi >= S::kSlots) ok = mbar_park_warp(&sm->empty[vi % S::kSlots], (vi / S::kSlots - 1) & 1, st, kStatusTimeout);
+      if (!ok) return;
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-          store_row(k_tile(s), i, kreg[i], T());
-          kreg[i] = load_row(a.k, row0, len, nb, i);
-        }
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-          store_row(v_tile(s), i, vreg[i], __half());
-          vreg[i] = load_row(a.v, row0, len, nb, i);
-        }
-        sreg = load_scale(row0, len, nb);
-        fence_async_smem();
-        mbar_arrive(&sm->full[s]);
+      for (int i = 0; i < L; ++i) {
+        store_row(slot(vi), i, r.v[i], __half());
+        r.v[i] = load_row(a.v, i);
       }
+      fence_async_smem();
+      mbar_arrive(&sm->full[vi % S::kSlots]);
+      --ahead;
+      advance();
+      ++gb;
+    };
+    open();
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        regs[u].k[i] = load_row(a.k, i);
+        regs[u].v[i] = load_row(a.v, i);
+      }
+      load_scales(regs[u]);
+      advance();
+    }
+    while (ok && ahead > 0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (ok && ahead > 0) convert(regs[u]);
     }
   } else {
     regs_down<kRegsMma>();
-    if (warp == 8 && lane == 0) {
+    if (warp == 12 && lane == 0) {
       // ---------------- MMA ----------------
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t id_s = umma_idesc_16(fmt, false, kTileRows, kBlock), id_o = umma_idesc_16(0, true, kTileRows, D);
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity & 1, st, kStatusTimeout); };
-      auto scores = [&](int s) {
-        const uint32_t q = smem_addr(smem), k = smem_addr(k_tile(s));
-  #pragma unroll
+      auto wait = [&](uint64_t* bar, uint32_t phase) { return mbar_park(bar, phase & 1, st, kStatusTimeout); };
+      auto filled = [&](uint32_t i) { return wait(&sm->full[i % S::kSlots], i / S::kSlots); };
+      auto scores = [&](int s, int q_tile, uint32_t i) {
+        const uint32_t q = smem_addr(smem + q_tile * S::kQ), k = smem_addr(slot(i));
+        tc_fence_after();
+#pragma unroll
         for (int d = 0; d < D / 16; ++d)
-          tc_mma_f16_ss(tmem + s * kBlock, umma_desc_sw128(q + (d / 4) * S::kQHalf + (d % 4) * 32, 16, 1024),
+          tc_mma_f16_ss(tmem + s * kTmemS, umma_desc_sw128(q + (d / 4) * S::kQHalf + (d % 4) * 32, 16, 1024),
                         umma_desc_sw128(k + (d / 4) * S::kKvHalf + (d % 4) * 32, 16, 1024), id_s, d > 0);
         tc_commit(&sm->s_full[s]);
       };
-      auto values = [&](int s, bool acc) {
-        const uint32_t v = smem_addr(v_tile(s));
-  #pragma unroll
-        for (int k = 0; k < kBlock / 16; ++k)
-          tc_mma_f16_ts(tmem_o, tmem + s * kBlock + 8 * k, umma_desc_sw128(v + 2048 * k, S::kKvHalf, 1024), id_o,
-                        acc || k > 0);
-        tc_commit(&sm->pv_done);
-        tc_commit(&sm->empty[s]);
-      };
-      uint32_t gb = 0, part = 0;
-      bool ok = true;
-      bool more = true;
-      while (more && ok) {
-        ok = wait(&sm->q_full, part) && wait(&sm->full[gb & 1], gb >> 1);
-        if (!ok) break;
+      auto values = [&](int s, uint32_t i, bool acc) {
+        const uint32_t v = smem_addr(slot(i));
         tc_fence_after();
-        scores(gb & 1);
-        const int nb = walk.b1 - walk.b0;
-        if (nb == 1) tc_commit(&sm->q_empty);
-        for (int b = 0; b < nb && ok; ++b, ++gb) {
-          if (b + 1 < nb) {
-            ok = wait(&sm->full[(gb + 1) & 1], (gb + 1) >> 1);
+#pragma unroll
+        for (int k = 0; k < kBlock / 16; ++k)
+          tc_mma_f16_ts(tmem + kTmemO + s * D, tmem + s * kTmemS + 8 * k, umma_desc_sw128(v + 2048 * k, S::kKvHalf, 1024),
+                        id_o, acc || k > 0);
+        tc_commit(&sm->pv_done[s]);
+      };
+      auto release = [&](uint32_t i) { tc_commit(&sm->empty[i % S::kSlots]); };
+      uint32_t gb = 0, done[2] = {0, 0};
+      bool ok = true;
+      for (uint32_t part = 0;; ++part) {
+        ok = wait(&sm->part_full[part % kParts], part / kParts);
+        if (!ok) break;
+        const int nb = sm->part[part % kParts].nb;
+        const bool dual = sm->part[part % kParts].dual;
+        if (nb == 0) break;
+        give_back(part);
+        const uint32_t i0 = 2 * gb;  // ring index of block j's K: i0 + 2 j, of its V: one more
+        ok = wait(&sm->q_full, part) && filled(i0);
+        if (!ok) break;
+        if (dual) {
+          scores(0, 0, i0);
+          scores(1, 1, i0);
+          release(i0);
+          if (nb == 1) tc_commit(&sm->q_empty);
+          for (int j = 0; j < nb && ok; ++j) {
+            const uint32_t vi = i0 + 2 * j + 1, kn = vi + 1;
+            const bool again = j + 1 < nb;
+            ok = filled(vi) && (!again || filled(kn));
+            for (int s = 0; s < 2 && ok; ++s) {
+              ok = (j > 0 || part == 0 || wait(&sm->o_free[s], part - 1)) && wait(&sm->p_full[s], done[s]);
+              if (!ok) break;
+              values(s, vi, j > 0);
+              ++done[s];
+              if (again) scores(s, s, kn);
+            }
             if (!ok) break;
-            tc_fence_after();
-            scores((gb + 1) & 1);
-            if (b + 2 == nb) tc_commit(&sm->q_empty);
+            release(vi);
+            if (again) release(kn);
+            if (j + 2 == nb) tc_commit(&sm->q_empty);
           }
-          if (b == 0 && part > 0) ok = wait(&sm->o_free, part - 1);
-          ok = ok && wait(&sm->p_full[gb & 1], gb >> 1);
-          if (!ok) break;
-          tc_fence_after();
-          values(gb & 1, b > 0);
+        } else {
+          scores(0, 0, i0);
+          release(i0);
+          if (nb > 1) {
+            ok = filled(i0 + 2);
+            if (!ok) break;
+            scores(1, 0, i0 + 2);
+            release(i0 + 2);
+          }
+          if (nb <= 2) tc_commit(&sm->q_empty);
+          for (int j = 0; j < nb && ok; ++j) {
+            const int s = j & 1;
+            const uint32_t vi = i0 + 2 * j + 1, kn = vi + 3;
+            ok = filled(vi) && (j > 1 || part == 0 || wait(&sm->o_free[s], part - 1)) && wait(&sm->p_full[s], done[s]);
+            if (!ok) break;
+            values(s, vi, j > 1);
+            ++done[s];
+            release(vi);
+            if (j + 2 < nb) {
+              ok = filled(kn);
+              if (!ok) break;
+              scores(s, 0, kn);
+              release(kn);
+              if (j + 3 == nb) tc_commit(&sm->q_empty);
+            }
+          }
         }
-        ++part;
-        more = walk.next(a, w, G);
+        if (!ok) break;
+        gb += nb;
       }
       if (!ok) {  // let what was issued end before TMEM and shared memory go
         tc_commit(&sm->q_empty);
-        mbar_wait(&sm->q_empty, 0, nullptr, 0);
-        mbar_wait(&sm->q_empty, 1, nullptr, 0);
+        mbar_park(&sm->q_empty, 0, nullptr, 0);
+        mbar_park(&sm->q_empty, 1, nullptr, 0);
+      }
+    } else if (warp == 13) {
+      // ---------------- parts ----------------
+      Walk walk;
+      Part p = walk.begin(a, w, blockIdx.x, G, lane);
+      for (uint32_t i = 0;; ++i) {
+        if (i >= kParts && !mbar_park_warp(&sm->part_empty[i % kParts], (i / kParts - 1) & 1, st, kStatusTimeout)) break;
+        if (lane == 0) {
+          sm->part[i % kParts] = p;
+          mbar_arrive(&sm->part_full[i % kParts]);
+        }
+        __syncwarp();
+        if (p.nb == 0) break;
+        p = walk.next(a, w, blockIdx.x, G);
+      }
+    } else if (warp > 13) {
+      // ---------------- Q ----------------
+      bool ok = true;
+      for (uint32_t part = 0;; ++part) {
+        const Part& pt = take(part, ok);
+        if (!ok || pt.nb == 0) break;
+        if (part > 0) ok = mbar_park_warp(&sm->q_empty, (part - 1) & 1, st, kStatusTimeout);
+        if (!ok) break;
+        const int rows = pt.nt * G, first = pt.dual ? half * G : rows, tiles = pt.dual ? 2 : 1;
+        const T* q0 = static_cast<const T*>(a.q) + static_cast<int64_t>(pt.t0) * a.q_ld + static_cast<int64_t>(pt.kv) * G * D;
+        for (int i = threadIdx.x - 448; i < tiles * kTileRows * (D / 8); i += 64) {
+          const int r = i / (D / 8), c = i % (D / 8), tile = r / kTileRows, q = r % kTileRows;
+          uint8_t* dst = smem + tile * S::kQ + (c / 8) * S::kQHalf + q * 128 + (((c % 8) ^ (q & 7)) * 16);
+          if (q < (tile ? rows - first : first)) {
+            const int at = tile * first + q;
+            cp_async16(dst, q0 + static_cast<int64_t>(at / G) * a.q_ld + static_cast<int64_t>(at % G) * D + 8 * c);
+          } else {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);  // rows without a token
+          }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_smem();
+        mbar_arrive(&sm->q_full);
+        __syncwarp();
+        if (lane == 0) give_back(part);
       }
     }
   }
@@ -685,7 +876,7 @@ __global__ void __launch_bounds__(kAttendThreads, kCtasPerSm) k_shared_attend(Sh
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, S::kTmem);
+  if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
 // ---------------- join ----------------
@@ -694,62 +885,116 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
   constexpr int N = D / 32;  // values of a lane
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  pdl_wait();
   if (id >= static_cast<int64_t>(a.n) * a.H) return;
   const int t = static_cast<int>(id / a.H), h = static_cast<int>(id % a.H), G = a.H / a.KV, kv = h / G;
   const PlanHead head = *w.head;
   float m = -INFINITY, l = 0.0f, o[N] = {};
+  auto values = [&](const float* p, float (&v)[N]) {
+    if constexpr (N == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p);
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else {
+      const float2 q = *reinterpret_cast<const float2*>(p);
+      v[0] = q.x, v[1] = q.y;
+    }
+  };
   if (head.total > 0) {
+    // first partial row, distance of the next one and count, of the prefix's and of the own tile
+    int64_t r0[2] = {0, 0}, dist[2] = {0, 0};
+    int n[2] = {0, 0};
+#pragma unroll
     for (int which = 0; which < 2; ++which) {
       const int i = which ? w.tok_own[t] : w.tok_pre[t];
       if (i < 0) continue;
       const Tile x = w.tile[i];
       if (x.blocks == 0) continue;
-      const int64_t first = x.first + static_cast<int64_t>(kv) * x.blocks;
-      const int pieces = static_cast<int>((first + x.blocks - 1) / head.per - first / head.per) + 1;
-      const int64_t rows = static_cast<int64_t>(x.nt) * G;
-      const int64_t r0 = x.row + kv * pieces_bound(x.blocks, head.per) * rows + (t - x.t0) * G + h % G;
-      for (int p = 0; p < pieces; ++p) {
-        const int64_t r = r0 + p * rows;
-        const float2 ml = w.ml[r];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-        const float top = fmaxf(m, ml.x);
-        const float f = ex2_approx(m - top), g = ex2_approx(ml.x - top);
-        m = top;
-        l = l * f + ml.y * g;
+      const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
+      n[which] = static_cast<int>((first + x.places - 1) / head.per - first / head.per) + 1;
+      dist[which] = static_cast<int64_t>(x.nt) * G;
+      r0[which] = x.row + kv * pieces_bound(x.places, head.per) * dist[which] + (t - x.t0) * G + h % G;
+    }
+    for (int p0 = 0; p0 < n[0] + n[1]; p0 += 32) {  // a lane per piece, then the pieces' rows, four at a time
+      const int p = p0 + lane, all = min(32, n[0] + n[1] - p0);
+      int64_t r = 0;
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (p < n[0] + n[1]) {
+        r = p < n[0] ? r0[0] + p * dist[0] : r0[1] + (p - n[0]) * dist[1];
+        ml = w.ml[r];
+      }
+      const float top = fmaxf(m, warp_max(ml.x));
+      const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
+      const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ex2_approx(ml.x - top);
+      l = l * old + warp_sum(f == 0.0f ? 0.0f : f * ml.y);
+      m = top;
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = o[e] * f + w.o[r * D + N * lane + e] * g;
+      for (int e = 0; e < N; ++e) o[e] *= old;
+      for (int q = 0; q < all; q += 4) {
+        float v[4][N], g[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int src = min(q + u, all - 1);
+          const int64_t rr = __shfl_sync(0xffffffffu, r, src);
+          g[u] = q + u < all ? __shfl_sync(0xffffffffu, f, src) : 0.0f;
+          values(w.o + rr * D + N * lane, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] += g[u] * v[u][e];
       }
     }
   }
-  // ancestors
+  // ancestors, four at a time
   if (a.anc_off) {
     const int lo = a.anc_off[t], hi = a.anc_off[t + 1];
     const int64_t base = a.kv_base[t];
     bool bad = lo < 0 || hi < lo || hi > a.n_anc;
-    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(t) * a.q_ld + static_cast<int64_t>(h) * D + N * lane;
-    float qv[N];
+    if (!bad && lo < hi) {
+      const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(t) * a.q_ld + static_cast<int64_t>(h) * D + N * lane;
+      float qv[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) qv[e] = to_float(q[e]);
-    for (int i = lo; i < hi && !bad; ++i) {
-      const int64_t r = base + a.anc[i];
-      if (a.anc[i] < 0 || base < 0 || r >= a.n_rows) {
-        bad = true;
-        break;
+      for (int e = 0; e < N; ++e) qv[e] = to_float(q[e]) * (a.scale * 1.44269504088896341f);
+      for (int i = lo; i < hi && !bad; i += 4) {
+        int64_t at[4];
+        int some = 0;  // of the four that are in the cache, up to the first that is not
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int64_t r = i + u < hi ? base + a.anc[i + u] : -1;
+          const bool in = i + u < hi && a.anc[i + u] >= 0 && base >= 0 && r < a.n_rows;
+          bad |= i + u < hi && !in;
+          if (in && !bad) ++some;
+          at[u] = static_cast<int64_t>(kv) * a.n_rows + (in ? r : 0);
+        }
+        float s[4], vs[4], v[4][N];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          s[u] = 0.0f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            s[u] += qv[e] * static_cast<float>(a.k[at[u] * D + N * lane + e]);
+            v[u][e] = static_cast<float>(a.v[at[u] * D + N * lane + e]);
+          }
+          vs[u] = a.vs[at[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = u < some ? warp_sum(s[u]) * a.ks[at[u]] : -INFINITY;
+        const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m);
+        const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] *= old;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (u < some) {
+            const float g = ex2_approx(s[u] - top);
+            l += g;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] += g * vs[u] * v[u][e];
+          }
+        }
       }
-      const int64_t at = static_cast<int64_t>(kv) * a.n_rows + r;
-      const int8_t* k = a.k + at * D + N * lane;
-      const int8_t* v = a.v + at * D + N * lane;
-      float s = 0.0f;
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += qv[e] * static_cast<float>(k[e]);
-      s = warp_sum(s) * (a.ks[at] * (a.scale * 1.44269504088896341f));
-      const float top = fmaxf(m, s);
-      const float f = m == -INFINITY ? 0.0f : ex2_approx(m - top), g = ex2_approx(s - top);
-      m = top;
-      l = l * f + g;
-      const float gv = g * a.vs[at];
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = o[e] * f + gv * static_cast<float>(v[e]);
     }
     if (bad && lane == 0 && a.status) atomicCAS(a.status, 0, kStatusBadIndex);
   }
@@ -773,10 +1018,10 @@ int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
     cudaFuncAttributes at;
     e = cudaFuncGetAttributes(&at, k_shared_attend<T, D>);
     if (e != cudaSuccess) return e;
-    if (at.numRegs * 3 < kRegsSoftmax + kRegsConvert + kRegsMma) return cudaErrorInvalidConfiguration;
+    if (at.numRegs * 4 < 2 * kRegsSoftmax + kRegsConvert + kRegsMma) return cudaErrorInvalidConfiguration;
     set[dev] = true;
   }
-  const int ctas = kCtasPerSm * sms;
+  const int ctas = sms;
   const WsLayout y = ws_layout(a.n, a.H, a.KV, D, a.n_groups, ctas);
   uint8_t* p = static_cast<uint8_t*>(ws);
   SharedWs w{reinterpret_cast<PlanHead*>(p + y.head), reinterpret_cast<Tile*>(p + y.tile),
@@ -785,16 +1030,20 @@ int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
              reinterpret_cast<float*>(p + y.o),       y.rows,
              static_cast<int>(y.prefix_tiles)};
   k_shared_plan<<<1, kPlanThreads, 0, s>>>(a, w, ctas);
-  k_shared_attend<T, D><<<ctas, kAttendThreads, shared_smem<D>(), s>>>(a, w);
+  e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_pdl(k_shared_attend<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(kAttendThreads), shared_smem<D>(), s, 1,
+                   a, w);
   const int64_t warps = static_cast<int64_t>(a.n) * a.H;
-  k_shared_join<T, D><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, s>>>(a, w);
-  return cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_pdl(k_shared_join<T, D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, s, 1, a, w);
+  return e;
 }
 
 }  // namespace
 
 int64_t attention_shared_workspace(int n, int H, int KV, int D, int n_groups, int sms) {
-  return ws_layout(n, H, KV, D, n_groups, kCtasPerSm * sms).bytes;
+  return ws_layout(n, H, KV, D, n_groups, sms).bytes;
 }
 
 int launch_attention_shared(const SharedArgs& a, ActType type, int D, void* ws, int sms, cudaStream_t s) {

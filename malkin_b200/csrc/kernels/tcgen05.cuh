@@ -140,6 +140,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// The larger of three (one instruction on sm_100); NaN only if all are.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // Register split of a warpgroup (every warp of the group executes it; the groups' shares sum to at most the launch's).
 template <int N>
 __device__ __forceinline__ void regs_up() {

@@ -16,7 +16,7 @@
 // A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the
 // row's exponentials and sums are in 64 bits: with 32 the drawn index would differ from the exact one about once in 10^4
 // draws. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
-// slower: 93, 85 and 96 us against YY us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
+// slower: 93, 85 and 96 us against 72 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,6 +27,7 @@
 #include "common.cuh"
 #include "kernels.hpp"
 #include "pdl.cuh"
+#include "tcgen05.cuh"
 #include "types16.cuh"
 
 namespace mkb {
@@ -34,11 +35,9 @@ namespace mkb {
 namespace {
 
 constexpr int kRowThreads = 256;
-// A thread holds 64 bytes of a row at a time; a tile is what a block holds.
-template <typename T>
-constexpr int kRowVals = 64 / sizeof(T);
-template <typename T>
-constexpr int kRowTile = kRowThreads * kRowVals<T>;
+constexpr int kRowVals = 16;                        // logits a thread holds at a time
+constexpr int kRowTile = kRowThreads * kRowVals;    // 4096
+constexpr int kRowTilesMax = 8;                     // of a CTA
 constexpr int kDrawThreads = 256, kDrawVals = 16;   // of the normalisation and the rest
 constexpr int kDrawChunk = kDrawThreads * kDrawVals;
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
@@ -58,20 +57,17 @@ struct Decision {  // of a request
   double c, u;     // log2 e / T, the draw's uniform
 };
 
-template <typename T>
 int verify_chunk_tiles(int n_rows, int V, int sms) {
-  // one tile per CTA while that gives fewer than 8 CTAs per SM, else up to four tiles (fewer, longer CTAs)
-  const int64_t tiles = (static_cast<int64_t>(V) + kRowTile<T> - 1) / kRowTile<T>;
-  const int64_t per = tiles * n_rows / (8 * static_cast<int64_t>(sms));
-  return static_cast<int>(per < 1 ? 1 : per > 4 ? 4 : per);
+  // as many tiles a CTA as give four CTAs per SM, one wave, in which the next tile's loads run under this one's work
+  const int64_t tiles = (static_cast<int64_t>(V) + kRowTile - 1) / kRowTile;
+  const int64_t per = (tiles * n_rows + 4 * sms - 1) / (4 * sms);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(per, kRowTilesMax)));
 }
 
 __device__ __forceinline__ bool above(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
 
-// One 16-byte word of logits as floats.
 template <typename T>
-__device__ __forceinline__ void load16b(const T* p, float* v) {
-  const uint4 q = ld_stream16(p);
+__device__ __forceinline__ void unpack16b(uint4 q, float* v) {
   if constexpr (sizeof(T) == 4) {
     v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
   } else {
@@ -85,29 +81,30 @@ __device__ __forceinline__ void load16b(const T* p, float* v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int tiles, int n_chunks, RowPart* parts) {
-  constexpr int W = 16 / sizeof(T);  // values per word
-  constexpr int kVals = kRowVals<T>, kTile = kRowTile<T>;
+__global__ void __launch_bounds__(kRowThreads, 4) k_verify_rows(VerifyArgs a, int tiles, int n_chunks, RowPart* parts) {
+  constexpr int W = 16 / sizeof(T), N = kRowVals / W;  // values of a word, words of a thread
   __shared__ float s_mx[kRowThreads / 32];
   __shared__ int s_idx[kRowThreads / 32];
   __shared__ double s_sum[kRowThreads / 32];
   const int row = blockIdx.x, chunk = blockIdx.y, tid = threadIdx.x;
   const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld;
-  const int64_t begin = static_cast<int64_t>(chunk) * tiles * kTile;
-  const int64_t end = min(begin + static_cast<int64_t>(tiles) * kTile, static_cast<int64_t>(a.V));
+  const int64_t begin = static_cast<int64_t>(chunk) * tiles * kRowTile;
+  const int64_t end = min(begin + static_cast<int64_t>(tiles) * kRowTile, static_cast<int64_t>(a.V));
   // rows whose address is not a multiple of 16 are read value by value
   const bool vec = (reinterpret_cast<uintptr_t>(l) & 15) == 0;
   pdl_launch();
-  float v[kVals];
-  auto load = [&](int64_t at) {  // tile `at`: W-value words, kRowThreads apart; absent values are -inf
+  uint4 raw[N];
+  auto load = [&](int64_t at) {  // tile `at`: words kRowThreads apart; absent values are -inf
 #pragma unroll
-    for (int b = 0; b < kVals / W; ++b) {
+    for (int b = 0; b < N; ++b) {
       const int64_t i = at + static_cast<int64_t>(b * kRowThreads + tid) * W;
       if (vec && i + W <= end) {
-        load16b<T>(l + i, v + b * W);
+        raw[b] = ld_stream16(l + i);
       } else {
+        alignas(16) T one[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[b * W + e] = i + e < end ? to_float(l[i + e]) : -INFINITY;
+        for (int e = 0; e < W; ++e) one[e] = i + e < end ? l[i + e] : from_float<T>(-INFINITY);
+        raw[b] = *reinterpret_cast<const uint4*>(one);
       }
     }
   };
@@ -117,31 +114,31 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
   for (int r0 = 0; r0 < a.n_req; r0 += kRowThreads)
     before += __syncthreads_count(r0 + tid < a.n_req && a.row_off[r0 + tid + 1] <= row);
   const float T0 = before < a.n_req ? a.temperature[before] : 0.0f;
-  const bool sums = T0 > 0.0f;                                      // greedy rows need no sum
+  const bool sums = T0 > 0.0f;  // rows of a greedy request need the index of the maximum, the others the sum
   const float c = sums ? fminf(1.44269504088896341f / T0, FLT_MAX) : 0.0f;  // exp(x / T) = 2^(x c)
   float mx = -INFINITY, sum = 0.0f;
   int idx = INT32_MAX;
-  for (int64_t at = begin;;) {
-    float m = -INFINITY;
+  for (int64_t at = begin; at < end; at += kRowTile) {
+    float v[kRowVals];
 #pragma unroll
-    for (int e = 0; e < kVals; ++e) {
-      v[e] = fmaxf(v[e], -INFINITY);  // NaN reads as -inf
-      m = fmaxf(m, v[e]);
-    }
+    for (int b = 0; b < N; ++b) unpack16b<T>(raw[b], v + b * W);
+    if (at + kRowTile < end) load(at + kRowTile);
+    float m = -INFINITY;  // fmaxf passes over NaN
+#pragma unroll
+    for (int e = 0; e < kRowVals; ++e) m = fmaxf(m, v[e]);
     if (m > mx) {
-      sum = mx > -INFINITY ? sum * exp2f((mx - m) * c) : 0.0f;
+      sum = mx > -INFINITY ? sum * ex2_approx((mx - m) * c) : 0.0f;
       mx = m;
+      if (!sums) {
 #pragma unroll
-      for (int e = kVals - 1; e >= 0; --e)
-        if (v[e] == m) idx = static_cast<int>(at + static_cast<int64_t>((e / W) * kRowThreads + tid) * W + e % W);
+        for (int e = kRowVals - 1; e >= 0; --e)
+          if (v[e] == m) idx = static_cast<int>(at + static_cast<int64_t>((e / W) * kRowThreads + tid) * W + e % W);
+      }
     }
     if (mx > -INFINITY && sums) {
 #pragma unroll
-      for (int e = 0; e < kVals; ++e) sum += exp2f((v[e] - mx) * c);
+      for (int e = 0; e < kRowVals; ++e) sum += ex2_approx((fmaxf(v[e], -INFINITY) - mx) * c);
     }
-    at += kTile;
-    if (at >= end) break;
-    load(at);
   }
   // join the block: maximum and index first, then the sums at that maximum
   float bm = mx;
@@ -152,18 +149,27 @@ __global__ void __launch_bounds__(kRowThreads) k_verify_rows(VerifyArgs a, int t
     const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
     if (above(om, oi, bm, bi)) bm = om, bi = oi;
   }
-  double s = mx > -INFINITY ? static_cast<double>(sum * exp2f((mx - bm) * c)) : 0.0;
+  double s = mx > -INFINITY ? static_cast<double>(sum * ex2_approx((mx - bm) * c)) : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((tid & 31) == 0) s_mx[tid >> 5] = bm, s_idx[tid >> 5] = bi, s_sum[tid >> 5] = s;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kRowThreads / 32; ++w)
-      if (above(s_mx[w], s_idx[w], bm, bi)) bm = s_mx[w], bi = s_idx[w];
-    double total = 0.0;
-    for (int w = 0; w < kRowThreads / 32; ++w)
-      if (s_mx[w] > -INFINITY) total += s_sum[w] * static_cast<double>(exp2f((s_mx[w] - bm) * c));
-    parts[static_cast<int64_t>(row) * n_chunks + chunk] = RowPart{bm, bi, total};
+  if (tid < 32) {
+    constexpr int kW = kRowThreads / 32;
+    const bool in = tid < kW;
+    const float wm = in ? s_mx[tid] : -INFINITY;
+    bm = wm;
+    bi = in ? s_idx[tid] : INT32_MAX;
+#pragma unroll
+    for (int o = kW / 2; o > 0; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, bm, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (above(om, oi, bm, bi)) bm = om, bi = oi;
+    }
+    double total = in && wm > -INFINITY ? s_sum[tid] * static_cast<double>(ex2_approx((wm - bm) * c)) : 0.0;
+#pragma unroll
+    for (int o = kW / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (tid == 0) parts[static_cast<int64_t>(row) * n_chunks + chunk] = RowPart{bm, bi, total};
   }
 }
 
@@ -250,9 +256,23 @@ struct Weigh {
   }
 };
 
+// A thread's values of one of the draw's chunks, kDrawThreads apart; `fill` past the row's end.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* row, int chunk, int V, T fill, T (&v)[kDrawVals]) {
+  const int j0 = chunk * kDrawChunk + static_cast<int>(threadIdx.x);  // V is at most 2^27
+  const T* p = row + j0;
+  if ((chunk + 1) * static_cast<int64_t>(kDrawChunk) <= V) {
+#pragma unroll
+    for (int g = 0; g < kDrawVals; ++g) v[g] = p[g * kDrawThreads];
+  } else {
+#pragma unroll
+    for (int g = 0; g < kDrawVals; ++g) v[g] = j0 + g * kDrawThreads < V ? p[g * kDrawThreads] : fill;
+  }
+}
+
 // Grid: (CTAs of a request, request); each takes `per` of the draw's chunks.
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) k_verify_norm(VerifyArgs a, int n_chunks, const RowPart* parts,
+__global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, int n_chunks, const RowPart* parts,
                                                               Decision* decide, double* zpart, int chunks, int per) {
   __shared__ double tab[16], part[kDrawThreads / 32];
   __shared__ int first;
@@ -334,28 +354,25 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_norm(VerifyArgs a, int 
   if (!d.draw) return;
   const T* l = logits + static_cast<int64_t>(row) * a.ld;
   const Weigh w(d, tab, a.q != nullptr);
-  float x[kDrawVals];
-  auto load = [&](int chunk) {
-#pragma unroll
-    for (int g = 0; g < kDrawVals; ++g) {
-      const int64_t j = static_cast<int64_t>(chunk) * kDrawChunk + g * kDrawThreads + tid;
-      x[g] = chunk < chunks && j < a.V ? to_float(l[j]) : -INFINITY;
-    }
-  };
+  T next[kDrawVals];
+  auto load = [&](int chunk) { load_chunk(l, chunk, a.V, from_float<T>(-INFINITY), next); };
   const int c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
   load(c0);
   for (int chunk = c0; chunk < c1; ++chunk) {
+    float x[kDrawVals];
+#pragma unroll
+    for (int g = 0; g < kDrawVals; ++g) x[g] = to_float(next[g]);
+    if (chunk + 1 < c1) load(chunk + 1);
     double v = 0.0;
 #pragma unroll
     for (int g = 0; g < kDrawVals; ++g) v += w.whole(x[g]);
-    if (chunk + 1 < c1) load(chunk + 1);
     v = block_sum(v, part);
     if (tid == 0) zpart[static_cast<int64_t>(r) * chunks + chunk] = v;
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) k_verify_rest(VerifyArgs a, const Decision* decide, const double* zpart,
+__global__ void __launch_bounds__(kDrawThreads, 4) k_verify_rest(VerifyArgs a, const Decision* decide, const double* zpart,
                                                               double* rpart) {
   __shared__ double tab[16], part[kDrawThreads / 32];
   const int r = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
@@ -367,20 +384,17 @@ __global__ void __launch_bounds__(kDrawThreads) k_verify_rest(VerifyArgs a, cons
   if (!d.draw || d.draft < 0) return;  // drawn from p itself: the shares are the normalisation's
   const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(d.row) * a.ld;
   const float* q = a.q ? a.q + static_cast<int64_t>(d.draft) * a.q_ld : nullptr;
-  float x[kDrawVals], y[kDrawVals];
-#pragma unroll
-  for (int g = 0; g < kDrawVals; ++g) {
-    const int64_t j = static_cast<int64_t>(chunk) * kDrawChunk + g * kDrawThreads + tid;
-    x[g] = j < a.V ? to_float(l[j]) : -INFINITY;
-    y[g] = q && j < a.V ? q[j] : 0.0f;
-  }
+  T x[kDrawVals];
+  float y[kDrawVals] = {};
+  load_chunk(l, chunk, a.V, from_float<T>(-INFINITY), x);
+  if (q) load_chunk(q, chunk, a.V, 0.0f, y);
   Weigh w(d, tab, q != nullptr);
   double z = 0.0;
   for (unsigned i = tid; i < gridDim.x; i += kDrawThreads) z += zpart[static_cast<int64_t>(r) * gridDim.x + i];
   w.Z = block_sum(z, part);
   double v = 0.0;
 #pragma unroll
-  for (int g = 0; g < kDrawVals; ++g) v += w.rest(chunk * kDrawChunk + g * kDrawThreads + tid, x[g], y[g]);
+  for (int g = 0; g < kDrawVals; ++g) v += w.rest(chunk * kDrawChunk + g * kDrawThreads + tid, to_float(x[g]), y[g]);
   v = block_sum(v, part);
   if (tid == 0) rpart[static_cast<int64_t>(r) * gridDim.x + chunk] = v;
 }
@@ -496,7 +510,7 @@ VerifyWs verify_ws(int n_rows, int n_req, int V) {
     return p;
   };
   // chunks of one tile are the most a row can have
-  w.parts = take((static_cast<int64_t>(V) + kRowTile<float> - 1) / kRowTile<float> * n_rows * static_cast<int64_t>(sizeof(RowPart)));
+  w.parts = take((static_cast<int64_t>(V) + kRowTile - 1) / kRowTile * n_rows * static_cast<int64_t>(sizeof(RowPart)));
   w.chunks = (static_cast<int64_t>(V) + kDrawChunk - 1) / kDrawChunk;
   w.decide = take(n_req * static_cast<int64_t>(sizeof(Decision)));
   w.zpart = take(n_req * w.chunks * 8);
@@ -507,9 +521,9 @@ VerifyWs verify_ws(int n_rows, int n_req, int V) {
 
 template <typename T>
 int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
-  const int tiles = verify_chunk_tiles<T>(a.n_rows, a.V, sms);
-  const int n_chunks = static_cast<int>((static_cast<int64_t>(a.V) + static_cast<int64_t>(tiles) * kRowTile<T> - 1) /
-                                        (static_cast<int64_t>(tiles) * kRowTile<T>));
+  const int tiles = verify_chunk_tiles(a.n_rows, a.V, sms);
+  const int n_chunks = static_cast<int>((static_cast<int64_t>(a.V) + static_cast<int64_t>(tiles) * kRowTile - 1) /
+                                        (static_cast<int64_t>(tiles) * kRowTile));
   const VerifyWs y = verify_ws(a.n_rows, a.n_req, a.V);
   uint8_t* p = static_cast<uint8_t*>(a.ws);
   RowPart* parts = reinterpret_cast<RowPart*>(p + y.parts);
@@ -520,7 +534,7 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
       a, tiles, n_chunks, parts);
   cudaError_t e = cudaGetLastError();
   const dim3 grid(static_cast<unsigned>(y.chunks), static_cast<unsigned>(a.n_req));
-  // every CTA of a request walks its drafts again, so a request gets no more CTAs than fill the SMs four times over
+  // every CTA of a request walks its drafts again, so requests get no more CTAs than the SMs hold at once
   const int most = std::max(1, 4 * sms / a.n_req), per = static_cast<int>((y.chunks + most - 1) / most);
   const dim3 walk(static_cast<unsigned>((y.chunks + per - 1) / per), static_cast<unsigned>(a.n_req));
   if (e == cudaSuccess)
