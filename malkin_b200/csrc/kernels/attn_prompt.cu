@@ -7,9 +7,9 @@
 //
 // A CTA takes 256 rows of one head as two tiles of 128, so each K / V tile read from L2 feeds two tiles, and one tile's
 // MMAs run while the other's softmax does:
-//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread per row; S from TMEM, P back over S (16-bit, half the columns)
-//   warps 8-11       O *= exp(m_old - m_new) when a row's maximum grew, then the epilogue of both tiles
-//   warp 12          issues every MMA      warp 13  TMA loads     warps 14, 15  check the V tiles of the diagonal
+//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread per row; S from TMEM, P back over S (16-bit, half the columns),
+//                    O *= exp(m_old - m_new) when a row's maximum grew, the epilogue
+//   warp 8           issues every MMA      warp 9  TMA loads     warps 10, 11  check the V tiles of the diagonal
 // TMEM (512 columns): S0 | S1 | O0 | O1. Shared memory: both Q tiles and a ring of K and V tiles of 128 keys.
 //
 // The maximum used for a row is only raised when it grew by more than 8 in the exponent of 2 (weights stay below 2^8,
@@ -40,7 +40,8 @@ namespace {
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kPair = 256;   // rows of a CTA
 constexpr int kKeys = 128;   // keys of a block
-constexpr int kPromptThreads = 512;
+constexpr int kPromptThreads = 384;
+constexpr int kPromptSoftmaxRegs = 208, kPromptOtherRegs = 88;  // 2 x 208 + 88 = 3 x the 168 of the launch
 constexpr float kRaise = 8.0f;
 
 template <int D>
@@ -52,9 +53,7 @@ struct PromptShape {
 };
 
 struct PromptSmall {  // behind the tiles
-  uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2], sc_full[2], o_ready[2], pv_done[2], fin[2], go[2], clean[2];
-  float scale[2][kRows];
-  float sum[2][kRows];
+  uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2], pv_done[2], go[2], clean[2];
   uint32_t tmem;
   int seq_lo, seq_hi, tile;
   int odd_v;  // a diagonal V tile held an entry that is not finite
@@ -65,10 +64,12 @@ constexpr int prompt_smem() {
   return PromptShape<D>::kSmall + static_cast<int>(sizeof(PromptSmall));
 }
 
-// The sequence and the 256-row tile `want` (counted sequence after sequence, a sequence's longest tile first) belongs to.
+// The sequence and the 256-row tile that CTA `want` of a head takes: of each 32 sequences the tiles with the most keys first,
+// so that what runs last is short (in sequence order the eight packed prompts of the table took YY us for XX). A tile's place
+// is found from the number of tiles at or above a depth, by bisection.
 __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, int want, int lane, int* status,
                                           PromptSmall* sm) {
-  int base = 0, lo_f = 0, hi_f = 0, tile_f = -1;
+  int lo_f = 0, hi_f = 0, tile_f = -1;
   for (int s0 = 0; s0 < n_seq; s0 += 32) {
     const int s = s0 + lane;
     int lo = 0, hi = 0;
@@ -81,22 +82,25 @@ __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, 
       }
     }
     const int tiles = (hi - lo + kPair - 1) / kPair;
-    int incl = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
+    const int all = warp_isum(tiles);
+    if (want >= all) {
+      want -= all;
+      continue;
     }
-    const int first = base + incl - tiles;
-    const unsigned hit = __ballot_sync(0xffffffffu, want >= first && want < first + tiles);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      lo_f = __shfl_sync(0xffffffffu, lo, src);
-      hi_f = __shfl_sync(0xffffffffu, hi, src);
-      tile_f = __shfl_sync(0xffffffffu, first + tiles - 1, src) - want;
-      break;
+    int d = 0, above = 0;  // the deepest level with more than `want` tiles at or below it in the order; tiles deeper still
+    for (int top = __reduce_max_sync(0xffffffffu, tiles); top - d > 1;) {
+      const int mid = (d + top) / 2, at = warp_isum(max(0, tiles - mid));
+      if (at > want)
+        d = mid;
+      else
+        top = mid;
     }
-    base += __shfl_sync(0xffffffffu, incl, 31);
+    above = warp_isum(max(0, tiles - d - 1));
+    const int src = static_cast<int>(__fns(__ballot_sync(0xffffffffu, tiles > d), 0, want - above + 1));
+    lo_f = __shfl_sync(0xffffffffu, lo, src);
+    hi_f = __shfl_sync(0xffffffffu, hi, src);
+    tile_f = d;
+    break;
   }
   if (lane == 0) {
     sm->seq_lo = lo_f;
@@ -121,16 +125,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = static_cast<int>(blockIdx.x % a.H), want = static_cast<int>(blockIdx.x / a.H);
   if (warp == 0) find_tile(a.off, a.n_seq, a.n, want, lane, a.status, sm);
-  if (warp == 12) tmem_alloc(&sm->tmem, 512);
+  if (warp == 8) tmem_alloc(&sm->tmem, 512);
   if (threadIdx.x == 32) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm->q_full[t], 1);
       mbar_init(&sm->s_full[t], 1);
       mbar_init(&sm->p_full[t], 4);
-      mbar_init(&sm->sc_full[t], 4);
-      mbar_init(&sm->o_ready[t], 4);
       mbar_init(&sm->pv_done[t], 1);
-      mbar_init(&sm->fin[t], 4);
       mbar_init(&sm->go[t], 1);
       mbar_init(&sm->clean[t], 2);
     }
@@ -157,15 +158,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp < 8) {
     // ---------------- softmax ----------------
-    regs_up<192>();
+    regs_up<kPromptSoftmaxRegs>();
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const int blocks = t == 0 ? nb0 : nb1;
     const uint32_t ts = tmem + static_cast<uint32_t>(t * kKeys) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t to = tmem + static_cast<uint32_t>(2 * kKeys + t * D) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float c = a.scale * 1.44269504088896341f;  // exp(scale x) = 2^(c x)
     float m = -INFINITY, l = 0.0f;                   // maximum in use (of the raw scores), sum of the weights
     bool ok = true;
     for (int j = 0; j < blocks; ++j) {
-      ok = mbar_park_warp(&sm->s_full[t], j & 1, st, kStatusTimeout);
+      ok = mbar_wait_warp(&sm->s_full[t], j & 1, st, kStatusTimeout);
       if (!ok) break;
       tc_fence_after();
       float s[kKeys];
@@ -192,28 +194,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         scale = j == 0 ? 0.0f : ex2_approx((m - top) * c);
         m = top;
       }
-      if (j > 0) {
-        sm->scale[t][row] = scale;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm->sc_full[t]);
+      if (j > 0 && __any_sync(0xffffffffu, scale != 1.0f)) {
+        ok = mbar_wait_warp(&sm->pv_done[t], (j - 1) & 1, st, kStatusTimeout);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int b = 0; b < D / 32; ++b) {
+          uint32_t v[32];
+          tmem_ld32(to + 32 * b, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * scale);
+          tmem_st32(to + 32 * b, v);
+        }
       }
       const float mc = m == -INFINITY ? 0.0f : m * c;
       const f2 c2 = f2_make(c, c), m2 = f2_make(-mc, -mc);
       f2 sum2 = f2_make(0.0f, 0.0f), sum3 = sum2;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        uint32_t p[16];
+      for (int i = 0; i < kKeys; i += 2) {
+        const f2 x = f2_fma(f2_make(s[i], s[i + 1]), c2, m2);
+        s[i] = f2_lo(x);
+        s[i + 1] = f2_hi(x);
+      }
+      constexpr int kLag = 8;  // exponentials in flight
+      uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const f2 x = f2_fma(f2_make(s[32 * b + 2 * i], s[32 * b + 2 * i + 1]), c2, m2);
-          const float e0 = ex2_approx(f2_lo(x)), e1 = ex2_approx(f2_hi(x));
-          if (i & 1)
-            sum3 = f2_add(sum3, f2_make(e0, e1));
-          else
-            sum2 = f2_add(sum2, f2_make(e0, e1));
-          p[i] = pack2<T>(e0, e1);
+      for (int i = 0; i < kKeys + kLag; i += 2) {
+        if (i < kKeys) {
+          s[i] = ex2_approx(s[i]);
+          s[i + 1] = ex2_approx(s[i + 1]);
         }
-        tmem_st16(ts + 16 * b, p);
+        const int k = i - kLag;
+        if (k >= 0) {
+          if (k & 2)
+            sum3 = f2_add(sum3, f2_make(s[k], s[k + 1]));
+          else
+            sum2 = f2_add(sum2, f2_make(s[k], s[k + 1]));
+          p[(k / 2) & 15] = pack2<T>(s[k], s[k + 1]);
+          if ((k & 31) == 30) tmem_st16(ts + k / 32 * 16, p);
+        }
       }
       sum2 = f2_add(sum2, sum3);
       l = l * scale + (f2_lo(sum2) + f2_hi(sum2));
@@ -222,58 +242,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm->p_full[t]);
     }
+    if (ok && blocks > 0) ok = mbar_wait_warp(&sm->pv_done[t], (blocks - 1) & 1, st, kStatusTimeout);
     if (ok && blocks > 0) {
-      sm->sum[t][row] = l;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->fin[t]);
-    }
-  } else if (warp < 12) {
-    // ---------------- rescaling of O, epilogue ----------------
-    regs_down<80>();
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t to = tmem + 2 * kKeys + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    bool ok = true;
-    for (int j = 1; j < nb && ok; ++j) {
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (j >= (t == 0 ? nb0 : nb1)) continue;
-        ok = mbar_park_warp(&sm->sc_full[t], (j - 1) & 1, st, kStatusTimeout);
-        if (!ok) break;
-        const float f = sm->scale[t][row];
-        if (__any_sync(0xffffffffu, f != 1.0f)) {
-          ok = mbar_park_warp(&sm->pv_done[t], (j - 1) & 1, st, kStatusTimeout);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int b = 0; b < D / 32; ++b) {
-            uint32_t v[32];
-            tmem_ld32(to + t * D + 32 * b, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-            tmem_st32(to + t * D + 32 * b, v);
-          }
-          tmem_wait_st();
-          tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm->o_ready[t]);
-      }
-    }
-    for (int t = 0; t < 2 && ok; ++t) {
-      const int blocks = t == 0 ? nb0 : nb1;
-      if (blocks == 0) continue;
-      ok = mbar_park_warp(&sm->fin[t], 0, st, kStatusTimeout) &&
-           mbar_park_warp(&sm->pv_done[t], (blocks - 1) & 1, st, kStatusTimeout);
-      if (!ok) break;
       tc_fence_after();
-      const float inv = 1.0f / sm->sum[t][row];
+      const float inv = 1.0f / l;
       const int i = q0 + t * kRows + row;  // row in the sequence
       const bool odd = sm->odd_v != 0;     // written before the MMAs that pv_done stands for
       T* out = static_cast<T*>(a.out) + static_cast<int64_t>(lo + i) * a.out_ld + static_cast<int64_t>(head) * D;
 #pragma unroll 1
       for (int b = 0; b < D / 32; ++b) {
         uint32_t v[32];
-        tmem_ld32(to + t * D + 32 * b, v);
+        tmem_ld32(to + 32 * b, v);
         tmem_wait_ld();
         if (i < len) {
           float o[32];
@@ -303,69 +282,87 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
     }
   } else {
-    regs_down<48>();
-    if (warp == 12 && lane == 0) {
+    regs_down<kPromptOtherRegs>();
+    if (warp == 8) {
       // ---------------- MMA ----------------
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t id_s = umma_idesc_16(fmt, false, kRows, kKeys), id_o = umma_idesc_16(fmt, true, kRows, D);
-      auto wait = [&](uint64_t* bar, int parity) { return mbar_park(bar, parity & 1, st, kStatusTimeout); };
+      auto wait = [&](uint64_t* bar, int parity) { return mbar_wait_warp(bar, parity & 1, st, kStatusTimeout); };
+      // descriptors advance by their address field (in 16 bytes), which never carries out of it
+      const uint64_t q_desc = umma_desc_sw128(smem_addr(smem + S::kQ), 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(smem_addr(smem + S::kRing), 16, 1024);
+      const uint64_t v_desc = umma_desc_sw128(smem_addr(smem + S::kRing), S::kHalf, 1024);
       auto scores = [&](int t, int stage) {
-        const uint32_t q = smem_addr(smem + S::kQ + t * S::kTile), k = smem_addr(ring(stage));
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t q = q_desc + t * (S::kTile >> 4), k = k_desc + stage * (S::kTile >> 4);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          const uint32_t o = static_cast<uint32_t>((d / 4) * S::kHalf + (d % 4) * 32);
-          tc_mma_f16_ss(tmem + t * kKeys, umma_desc_sw128(q + o, 16, 1024), umma_desc_sw128(k + o, 16, 1024), id_s, d > 0);
+          for (int d = 0; d < D / 16; ++d) {
+            const int o = ((d / 4) * S::kHalf + (d % 4) * 32) >> 4;
+            tc_mma_f16_ss(tmem + t * kKeys, q + o, k + o, id_s, d > 0);
+          }
+          tc_commit(&sm->s_full[t]);
         }
-        tc_commit(&sm->s_full[t]);
+        __syncwarp();
       };
       auto values = [&](int t, int stage, bool acc) {
-        const uint32_t v = smem_addr(ring(stage));
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v = v_desc + stage * (S::kTile >> 4);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          tc_mma_f16_ts(tmem + 2 * kKeys + t * D, tmem + t * kKeys + 8 * k, umma_desc_sw128(v + 2048 * k, S::kHalf, 1024),
-                        id_o, acc || k > 0);
-        tc_commit(&sm->pv_done[t]);
+          for (int k = 0; k < kKeys / 16; ++k)
+            tc_mma_f16_ts(tmem + 2 * kKeys + t * D, tmem + t * kKeys + 8 * k, v + 128 * k, id_o, acc || k > 0);
+          tc_commit(&sm->pv_done[t]);
+        }
+        __syncwarp();
       };
-      auto stage = [&](int i) { return i % S::kStages; };
-      auto phase = [&](int i) { return i / S::kStages; };
+      auto release = [&](int stage) {
+        if (elect_one()) tc_commit(&sm->empty[stage]);
+        __syncwarp();
+      };
       bool ok = nb > 0;
       if (ok) {
-        ok = wait(&sm->full[0], 0);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if ((t == 0 ? nb0 : nb1) == 0) continue;
-          ok = wait(&sm->q_full[t], 0);
-          if (ok) {
-            tc_fence_after();
-            scores(t, 0);
-          }
+        ok = wait(&sm->full[0], 0) && wait(&sm->q_full[0], 0);
+        if (ok) scores(0, 0);
+        if (ok && nb1 > 0) {
+          ok = wait(&sm->q_full[1], 0);
+          if (ok) scores(1, 0);
         }
-        if (ok) tc_commit(&sm->empty[0]);
+        if (ok) release(0);
       }
+      int vs = 1, vp = 0, ks = 2, kp = 0;  // ring slots and phases of the block's V and of the next one's K
+      auto step = [&](int& slot, int& phase) {
+        slot += 2;
+        if (slot >= S::kStages) slot -= S::kStages, phase ^= 1;
+      };
       for (int j = 0; j < nb && ok; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
-        ok = wait(&sm->full[stage(vi)], phase(vi));
+        ok = wait(&sm->full[vs], vp);
         if (ok && j >= nb0 - 1) ok = wait(&sm->clean[j - (nb0 - 1)], 0);
-        if (ok && j + 1 < nb) ok = wait(&sm->full[stage(ki)], phase(ki));
-        for (int t = 0; t < 2 && ok; ++t) {
+        if (ok && j + 1 < nb) ok = wait(&sm->full[ks], kp);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
           const int blocks = t == 0 ? nb0 : nb1;
-          if (j >= blocks) continue;
-          ok = wait(&sm->p_full[t], j) && (j == 0 || wait(&sm->o_ready[t], j - 1));
-          if (!ok) break;
-          tc_fence_after();
-          values(t, stage(vi), j > 0);
-          if (j + 1 < blocks) scores(t, stage(ki));
+          if (j >= blocks || !ok) continue;
+          ok = wait(&sm->p_full[t], j);
+          if (!ok) continue;
+          values(t, vs, j > 0);
+          if (j + 1 < blocks) scores(t, ks);
         }
         if (ok) {
-          tc_commit(&sm->empty[stage(vi)]);
-          if (j + 1 < nb) tc_commit(&sm->empty[stage(ki)]);
+          release(vs);
+          if (j + 1 < nb) release(ks);
         }
+        step(vs, vp);
+        step(ks, kp);
       }
       if (!ok && nb > 0) {  // let what was issued end before TMEM and shared memory go
-        tc_commit(&sm->pv_done[0]);
-        mbar_park(&sm->pv_done[0], 0, nullptr, 0);
-        mbar_park(&sm->pv_done[0], 1, nullptr, 0);
+        if (elect_one()) tc_commit(&sm->pv_done[0]);
+        __syncwarp();
+        mbar_wait(&sm->pv_done[0], 0, nullptr, 0);
+        mbar_wait(&sm->pv_done[0], 1, nullptr, 0);
+        __syncwarp();
       }
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp == 9 && lane == 0) {
       // ---------------- loads ----------------
       auto load = [&](const CUtensorMap* map, uint8_t* dst, int h, int at, uint64_t* bar) {
         mbar_arrive_expect_tx(bar, S::kTile);
@@ -377,7 +374,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (nb0) load(&mq, smem + S::kQ, head, lo + q0, &sm->q_full[0]);
       for (int i = 0; i < 2 * nb && ok; ++i) {
         const int s = i % S::kStages, round = i / S::kStages;
-        if (round > 0) ok = mbar_park(&sm->empty[s], (round - 1) & 1, st, kStatusTimeout);
+        if (round > 0) ok = mbar_wait(&sm->empty[s], (round - 1) & 1, st, kStatusTimeout);
         if (!ok) break;
         load(i & 1 ? &mv : &mk, ring(s), kv, lo + (i / 2) * kKeys, &sm->full[s]);
         issued = i + 1;
@@ -386,21 +383,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       // every copy has landed before the block's shared memory goes
       for (int i = max(0, issued - S::kStages); i < issued; ++i)
-        mbar_park(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout);
-      if (nb0) mbar_park(&sm->q_full[0], 0, st, kStatusTimeout);
-      if (nb1 && issued) mbar_park(&sm->q_full[1], 0, st, kStatusTimeout);
-    } else if (warp >= 14 && nb > 0) {
+        mbar_wait(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout);
+      if (nb0) mbar_wait(&sm->q_full[0], 0, st, kStatusTimeout);
+      if (nb1 && issued) mbar_wait(&sm->q_full[1], 0, st, kStatusTimeout);
+    } else if (warp >= 10 && nb > 0) {
       // ---------------- V tiles whose keys some rows must not see ----------------
       for (int j = nb0 - 1; j < nb; ++j) {
         const int i = 2 * j + 1;
         // the load has been issued, so the stage's phase is this tile's; it is not reused before the tile is checked
-        if (!mbar_park_warp(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout) ||
-            !mbar_park_warp(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout))
+        if (!mbar_wait_warp_sleep(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout, 500) ||
+            !mbar_wait_warp(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout))
           break;
         uint4* v = reinterpret_cast<uint4*>(ring(i % S::kStages));
         bool seen = false;
 #pragma unroll 8
-        for (int x = (warp - 14) * 32 + lane; x < S::kTile / 16; x += 64) {
+        for (int x = (warp - 10) * 32 + lane; x < S::kTile / 16; x += 64) {
           const uint4 q = v[x];
           if (odd16<T>(q.x) || odd16<T>(q.y) || odd16<T>(q.z) || odd16<T>(q.w)) {
             alignas(16) T e[8];
@@ -423,7 +420,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int D>
@@ -441,11 +438,11 @@ int run_prompt(const PromptArgs& a, bool bf16, cudaStream_t s) {
   if (!set[dev]) {
     e = cudaFuncSetAttribute(k_attn_prompt<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prompt_smem<D>());
     if (e != cudaSuccess) return e;
-    // the warpgroups' register shares (2 x 192 + 80 + 48 for 128 threads each) come out of the launch's
+    // the warpgroups' register shares come out of the launch's
     cudaFuncAttributes at;
     e = cudaFuncGetAttributes(&at, k_attn_prompt<T, D>);
     if (e != cudaSuccess) return e;
-    if (at.numRegs * kPromptThreads < (2 * 192 + 80 + 48) * 128) return cudaErrorInvalidConfiguration;
+    if (at.numRegs * 3 < 2 * kPromptSoftmaxRegs + kPromptOtherRegs) return cudaErrorInvalidConfiguration;
     set[dev] = true;
   }
   // a sequence of L rows has at most L / 256 + 1 tiles

@@ -88,6 +88,14 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, 
       : "memory");
 }
 
+// One lane of a converged warp. The MMA warps run their loops as a whole and issue under this predicate, so that operand
+// descriptors stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t y;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(y));
+  return y != 0;
+}
+
 // Arrives once on bar when every tcgen05 operation this thread issued before has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
