@@ -109,10 +109,19 @@ __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, 
   }
 }
 
+// acc + 0 x each of the two values of w: NaN once a value that is not finite has been seen.
 template <typename T>
-__device__ __forceinline__ bool odd16(uint32_t w) {  // either half not finite
-  constexpr uint32_t E = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-  return (w & E) == E || ((w >> 16) & E) == E;
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t acc, uint32_t w);
+template <>
+__device__ __forceinline__ uint32_t add_zero_times<__half>(uint32_t acc, uint32_t w) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.0f), *reinterpret_cast<__half2*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t add_zero_times<__nv_bfloat16>(uint32_t acc, uint32_t w) {
+  __nv_bfloat162 r = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.0f),
+                             *reinterpret_cast<__nv_bfloat162*>(&acc));
+  return *reinterpret_cast<uint32_t*>(&r);
 }
 
 template <typename T, int D>
@@ -391,22 +400,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int j = nb0 - 1; j < nb; ++j) {
         const int i = 2 * j + 1;
         // the load has been issued, so the stage's phase is this tile's; it is not reused before the tile is checked
-        if (!mbar_wait_warp_sleep(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout, 500) ||
+        if (!mbar_wait_warp_sleep(&sm->go[j - (nb0 - 1)], 0, st, kStatusTimeout, 100) ||
             !mbar_wait_warp(&sm->full[i % S::kStages], (i / S::kStages) & 1, st, kStatusTimeout))
           break;
         uint4* v = reinterpret_cast<uint4*>(ring(i % S::kStages));
-        bool seen = false;
+        const int x0 = (warp - 10) * 32 + lane;
+        uint32_t acc[4] = {0, 0, 0, 0};
 #pragma unroll 8
-        for (int x = (warp - 10) * 32 + lane; x < S::kTile / 16; x += 64) {
+        for (int x = x0; x < S::kTile / 16; x += 64) {
           const uint4 q = v[x];
-          if (odd16<T>(q.x) || odd16<T>(q.y) || odd16<T>(q.z) || odd16<T>(q.w)) {
+          acc[0] = add_zero_times<T>(acc[0], q.x);
+          acc[1] = add_zero_times<T>(acc[1], q.y);
+          acc[2] = add_zero_times<T>(acc[2], q.z);
+          acc[3] = add_zero_times<T>(acc[3], q.w);
+        }
+        bool seen = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<T>(acc[e]);
+          seen |= f.x != f.x || f.y != f.y;
+        }
+        if (seen) {
+          for (int x = x0; x < S::kTile / 16; x += 64) {
             alignas(16) T e[8];
-            *reinterpret_cast<uint4*>(e) = q;
+            *reinterpret_cast<uint4*>(e) = v[x];
 #pragma unroll
             for (int y = 0; y < 8; ++y)
               if (!(fabsf(to_float(e[y])) < INFINITY)) e[y] = from_float<T>(0.0f);
             v[x] = *reinterpret_cast<const uint4*>(e);
-            seen = true;
           }
         }
         if (seen) sm->odd_v = 1;

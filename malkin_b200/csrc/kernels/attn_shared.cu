@@ -42,7 +42,7 @@ constexpr int kBlock = 96;         // keys: three pairs of K and V tiles and bot
 constexpr int kMinPiece = 2;       // places of the line in a CTA's piece; even, see Tile
 constexpr int kPlanThreads = 1024;
 constexpr int kAttendThreads = 512;  // warpgroups: softmax of stream 0, of stream 1, conversion, MMA and Q
-constexpr int kRegsSoftmax = 160, kRegsConvert = 104, kRegsMma = 88;  // 2 x 160 + 104 + 88 = 4 x the 128 of the launch
+constexpr int kRegsSoftmax = 176, kRegsConvert = 80, kRegsMma = 80;  // 2 x 176 + 80 + 80 = 4 x the 128 of the launch
 constexpr float kRaiseMax = 8.0f;   // a row's reference is raised when it is to grow by more (exponents of 2)
 constexpr float kHeadroom = 6.0f;   // of it below the largest weight x scale
 constexpr int kLeastExp = -40;      // of a block's largest V scale: blocks of zeros must not push the sums out of range
@@ -386,17 +386,19 @@ struct SharedShape {
   static constexpr int kQHalf = kTileRows * 128;  // bytes of 64 columns of a Q tile
   static constexpr int kKvHalf = kBlock * 128;    // of a K or V tile
   static constexpr int kQ = kHalves * kQHalf, kKv = kHalves * kKvHalf;
-  static constexpr int kRing = 2 * kQ, kSlots = 6, kSmall = kRing + kSlots * kKv;
+  static constexpr int kRing = 2 * kQ, kSlots = 5;
+  static constexpr int kRaws = 3, kRawTile = kBlock * D, kRaw = kRing + kSlots * kKv;  // int8 tiles as they come in
+  static constexpr int kSmall = kRaw + kRaws * kRawTile;
 };
-constexpr int kScaleSlots = 4;  // a block's scales are overwritten four blocks later, after its P V (the ring holds three)
-constexpr int kAhead = 1;       // blocks whose rows are in flight in the conversion warps' registers
+constexpr int kScaleSlots = 4;  // a block's scales are overwritten four blocks later, after the P V of the block after it
 constexpr int kParts = 4;       // parts known ahead
 struct SharedSmall {
   uint64_t part_full[kParts], part_empty[kParts];
-  uint64_t q_full, q_empty, full[6], empty[6], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
+  uint64_t q_full, q_empty, full[5], empty[5], raw_full[3], raw_empty[3], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
   alignas(16) float ks[kScaleSlots][kBlock];  // K scale x scale x log2 e
   alignas(16) float vs[kScaleSlots][kBlock];
   alignas(16) float vmax[kScaleSlots][4];     // largest finite |V scale| of each 32 keys of the block
+  uint32_t odd[kScaleSlots][4];   // those whose V scale is not finite, a bit each (the scale is kept as 0)
   Part part[kParts];
   float2 ml[kTileRows];           // stream 1's reference and sum, for stream 0 where they share the rows
   uint32_t tmem;
@@ -428,13 +430,17 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
     mbar_init(&sm->q_full, 64);
     for (int i = 0; i < kParts; ++i) {
       mbar_init(&sm->part_full[i], 1);
-      mbar_init(&sm->part_empty[i], 15);  // 8 softmax, 4 conversion and 2 Q warps, the MMA thread
+      mbar_init(&sm->part_empty[i], 15);  // 8 softmax, 4 conversion and 2 Q warps, the MMA warp
     }
     mbar_init(&sm->q_empty, 1);
     mbar_init(&sm->b_fin, 4);
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(&sm->full[i], 128);
       mbar_init(&sm->empty[i], 1);
+    }
+    for (int i = 0; i < S::kRaws; ++i) {
+      mbar_init(&sm->raw_full[i], 1);
+      mbar_init(&sm->raw_empty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm->s_full[i], 1);
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
   int* const st = a.status;
   // part i of the piece, once it is known; nb 0 (or a wait that ran out: ok false) ends the role's loop
   auto take = [&](uint32_t i, bool& ok) -> const Part& {
-    ok = mbar_park_warp(&sm->part_full[i % kParts], (i / kParts) & 1, st, kStatusTimeout);
+    ok = mbar_wait_warp(&sm->part_full[i % kParts], (i / kParts) & 1, st, kStatusTimeout);
     return sm->part[i % kParts];
   };
   auto give_back = [&](uint32_t i) { mbar_arrive(&sm->part_empty[i % kParts]); };
@@ -477,10 +483,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       if (row < rows) limit = pt.own ? own_keys(a, pt.t0 + (dual && s ? half : 0) + row / G, nullptr) : pt.len;
       limit -= pt.b0 * kBlock;
       float m = -INFINITY, l = 0.0f;
+      bool spoilt = false;  // this row sees a key whose V scale is not finite
       const int nb = pt.nb, step = dual ? 1 : 2, j0 = dual ? 0 : s;
       for (int j = j0; j < nb; j += step, ++mine) {
         const int sl = (gb + j) & (kScaleSlots - 1);
-        ok = mbar_park_warp(&sm->s_full[s], mine & 1, st, kStatusTimeout);
+        ok = mbar_wait_warp(&sm->s_full[s], mine & 1, st, kStatusTimeout);
         if (!ok) break;
         if (on) {
           tc_fence_after();
@@ -499,17 +506,28 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             const f2 y0 = f2_mul(f2_make(x[4 * i], x[4 * i + 1]), f2_make(k4.x, k4.y));
             const f2 y1 = f2_mul(f2_make(x[4 * i + 2], x[4 * i + 3]), f2_make(k4.z, k4.w));
             x[4 * i] = f2_lo(y0), x[4 * i + 1] = f2_hi(y0), x[4 * i + 2] = f2_lo(y1), x[4 * i + 3] = f2_hi(y1);
-            if (cut) {  // a masked key's scales may be anything
+          }
+          if (cut) {  // a branch of its own: selects on every score would cost as much as their exponentials
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (4 * i + e >= left) x[4 * i + e] = -INFINITY;
-            }
+            for (int i = 0; i < kBlock; ++i)
+              if (i >= left) x[i] = -INFINITY;
+          }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[4 * i + e]);
+          for (int i = 0; i < kBlock; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const float4 vm = *reinterpret_cast<const float4*>(sm->vmax[sl]);
           const float big = fmaxf(fmaxf(vm.x, vm.y), vm.z);
+          const uint32_t* odd = sm->odd[sl];
+          if (odd[0] | odd[1] | odd[2]) {
+#pragma unroll 1
+            for (int i = 0; i < 3; ++i) {
+              const int v = left - 32 * i;
+              spoilt |= (odd[i] & (v >= 32 ? 0xFFFFFFFFu : v <= 0 ? 0u : (1u << v) - 1)) != 0;
+            }
+          }
           const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, kLeastExp);
           const float want = top + (static_cast<float>(e) - kHeadroom);
           float scale = 1.0f;
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             m = want;
           }
           if (j > j0 && __any_sync(0xffffffffu, scale != 1.0f)) {
-            ok = mbar_park_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
+            ok = mbar_wait_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -546,10 +564,6 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
               const f2 e1 = f2_make(ex2_approx(f2_lo(y1)), ex2_approx(f2_hi(y1)));
               sum2 = f2_add(sum2, f2_add(e0, e1));
               f2 w0 = f2_mul(e0, f2_make(v4.x, v4.y)), w1 = f2_mul(e1, f2_make(v4.z, v4.w));
-              if (cut) {
-                w0 = f2_make(k < left ? f2_lo(w0) : 0.0f, k + 1 < left ? f2_hi(w0) : 0.0f);
-                w1 = f2_make(k + 2 < left ? f2_lo(w1) : 0.0f, k + 3 < left ? f2_hi(w1) : 0.0f);
-              }
               p[i] = pack2<__half>(f2_lo(w0), f2_hi(w0));
               p[i + 1] = pack2<__half>(f2_lo(w1), f2_hi(w1));
             }
@@ -563,14 +577,15 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         if (lane == 0) mbar_arrive(&sm->p_full[s]);
       }
       if (!ok) break;
+      if (spoilt) l = __int_as_float(0x7FFFFFFF);  // its output is NaN
       const int n_mine = dual ? nb : (nb + 1 - s) / 2, n_other = dual ? nb : nb - n_mine;
       other += n_other;
-      if (n_mine > 0) ok = mbar_park_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
+      if (n_mine > 0) ok = mbar_wait_warp(&sm->pv_done[s], (mine - 1) & 1, st, kStatusTimeout);
       if (!ok) break;
       tc_fence_after();
       if (!dual && s == 1) {
         // stream 0 has taken the last part's: with no block in this part, nothing else holds this stream back
-        if (part > 0) ok = mbar_park_warp(&sm->o_free[1], (part - 1) & 1, st, kStatusTimeout);
+        if (part > 0) ok = mbar_wait_warp(&sm->o_free[1], (part - 1) & 1, st, kStatusTimeout);
         if (!ok) break;
         sm->ml[row] = make_float2(m, l);
         tc_fence_before();
@@ -580,8 +595,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         float f0 = 1.0f, f1 = 0.0f;
         const bool join = !dual && n_other > 0;
         if (!dual) {
-          ok = mbar_park_warp(&sm->b_fin, splits & 1, st, kStatusTimeout) &&
-               (n_other == 0 || mbar_park_warp(&sm->pv_done[1], (other - 1) & 1, st, kStatusTimeout));
+          ok = mbar_wait_warp(&sm->b_fin, splits & 1, st, kStatusTimeout) &&
+               (n_other == 0 || mbar_wait_warp(&sm->pv_done[1], (other - 1) & 1, st, kStatusTimeout));
           if (!ok) break;
           tc_fence_after();
           const float2 o = sm->ml[row];
@@ -633,24 +648,16 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
     }
   } else if (warp < 12) {
     // ---------------- cache rows as 16-bit tiles ----------------
-    // thread: 16 int8 values (one load) at column block c4 of rows r, r + 32, r + 64, in each half of 64 columns. The eight
-    // threads of a store phase hold two rows x four blocks, which the swizzle spreads over all banks. The rows of the next
-    // block are in flight in registers.
+    // thread: 16 int8 values at column block c4 of rows r, r + 32, r + 64, in each half of 64 columns. The eight threads of a
+    // store phase hold two rows x four blocks, which the swizzle spreads over all banks.
     regs_down<kRegsConvert>();
     const int t = threadIdx.x - 256, c4 = t & 3, r0 = t >> 2;
-    constexpr int L = 3 * S::kHalves;  // loads of each of K and V
     const float kscale = a.scale * 1.44269504088896341f;
-    struct Rows {
-      uint4 k[L], v[L];
-      float ks, vs;
-    } regs[kAhead];
-    uint32_t gb = 0;
-    bool ok = true;
-    // the block whose rows are loaded next
-    uint32_t part = 0;
+    uint32_t gb = 0, part = 0;
+    bool ok = true, more = true;
     int64_t row0 = 0;
-    int len = 0, b = 0, end = 0, ahead = 0;  // ahead: blocks loaded and not yet stored
-    bool more = true;
+    int len = 0, b = 0, end = 0;  // the block whose scales are loaded next
+    float ks = 0.0f, vs = 0.0f;   // scales of the block that is stored next
     auto open = [&]() {
       const Part& pt = take(part, ok);
       more = ok && pt.nb > 0;
@@ -662,105 +669,103 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       if (more && lane == 0) give_back(part);
       ++part;
     };
-    auto load_row = [&](const int8_t* p, int i) {
-      const int key = b * kBlock + r0 + 32 * (i % 3);
-      if (!more || key >= len) return make_uint4(0, 0, 0, 0);
-      return ld_stream16(p + (row0 + key) * D + 64 * (i / 3) + 16 * c4);
-    };
-    auto load_scales = [&](Rows& r) {
+    auto load_scales = [&]() {
       const int key = b * kBlock + t;
-      const bool in = more && t < kBlock && key < len;
-      r.ks = in ? a.ks[row0 + key] * kscale : 0.0f;
-      r.vs = in ? a.vs[row0 + key] : 0.0f;
+      const bool in = t < kBlock && key < len;
+      ks = in ? a.ks[row0 + key] : 0.0f;
+      vs = in ? a.vs[row0 + key] : 0.0f;
     };
-    auto advance = [&]() {
-      if (!more) return;
-      ++ahead;
-      if (++b == end) open();
-    };
-    auto store_row = [&](uint8_t* tile, int i, uint4 v, auto tag) {
+    // tile i of the ring from the raw tile i
+    auto convert = [&](uint32_t i, auto tag) {
       using E = decltype(tag);
-      const int r = r0 + 32 * (i % 3);
-      uint8_t* base = tile + (i / 3) * S::kKvHalf + r * 128;
-      const uint2 a0 = widen4<E>(v.x), a1 = widen4<E>(v.y), a2 = widen4<E>(v.z), a3 = widen4<E>(v.w);
-      *reinterpret_cast<uint4*>(base + (((2 * c4) ^ (r & 7)) * 16)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
-      *reinterpret_cast<uint4*>(base + (((2 * c4 + 1) ^ (r & 7)) * 16)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
+      uint8_t* tile = slot(i);
+      const uint8_t* raw = smem + S::kRaw + (i % S::kRaws) * S::kRawTile + 16 * c4;
+#pragma unroll 1
+      for (int h = 0; h < S::kHalves; ++h) {
+        uint4 v[3];
+#pragma unroll
+        for (int u = 0; u < 3; ++u) v[u] = *reinterpret_cast<const uint4*>(raw + (r0 + 32 * u) * D + 64 * h);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+          const int r = r0 + 32 * u;
+          uint8_t* base = tile + h * S::kKvHalf + r * 128;
+          const uint2 a0 = widen4<E>(v[u].x), a1 = widen4<E>(v[u].y), a2 = widen4<E>(v[u].z), a3 = widen4<E>(v[u].w);
+          *reinterpret_cast<uint4*>(base + (((2 * c4) ^ (r & 7)) * 16)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
+          *reinterpret_cast<uint4*>(base + (((2 * c4 + 1) ^ (r & 7)) * 16)) = make_uint4(a2.x, a2.y, a3.x, a3.y);
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(&sm->full[i % S::kSlots]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm->raw_empty[i % S::kRaws]);
     };
-    auto convert = [&](Rows& r) {  // stores block gb, then loads the one kAhead blocks later into the same registers
-      const int sl = gb & (kScaleSlots - 1);
-      const uint32_t ki = 2 * gb, vi = 2 * gb + 1;
-      if (ki >= S::kSlots) ok = mbar_park_warp(&sm->empty[ki % S::kSlots], (ki / S::kSlots - 1) & 1, st, kStatusTimeout);
-      if (!ok) return;
-      if (t < kBlock) {
-        sm->ks[sl][t] = r.ks;
-        sm->vs[sl][t] = r.vs;
-        const float big = warp_max(fabsf(r.vs) < INFINITY ? fabsf(r.vs) : 0.0f);
-        if (lane == 0) sm->vmax[sl][t >> 5] = big;
-      }
-      load_scales(r);
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        store_row(slot(ki), i, r.k[i], T());
-        r.k[i] = load_row(a.k, i);
-      }
-      fence_async_smem();
-      mbar_arrive(&sm->full[ki % S::kSlots]);
-      if (vi >= S::kSlots) ok = mbar_park_warp(&sm->empty[vi % S::kSlots], (vi / S::kSlots - 1) & 1, st, kStatusTimeout);
-      if (!ok) return;
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        store_row(slot(vi), i, r.v[i], __half());
-        r.v[i] = load_row(a.v, i);
-      }
-      fence_async_smem();
-      mbar_arrive(&sm->full[vi % S::kSlots]);
-      --ahead;
-      advance();
-      ++gb;
+    auto ready = [&](uint32_t i) {  // the raw tile is there and the ring's slot is free
+      ok = mbar_wait_warp(&sm->raw_full[i % S::kRaws], (i / S::kRaws) & 1, st, kStatusTimeout) &&
+           (i < S::kSlots ||
+            mbar_wait_warp_sleep(&sm->empty[i % S::kSlots], (i / S::kSlots - 1) & 1, st, kStatusTimeout, 40));
+      return ok;
     };
     open();
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        regs[u].k[i] = load_row(a.k, i);
-        regs[u].v[i] = load_row(a.v, i);
+    if (more) load_scales();
+    while (more) {
+      const int sl = gb & (kScaleSlots - 1);
+      if (!ready(2 * gb)) break;
+      if (t < kBlock) {
+        const bool fine = fabsf(vs) < INFINITY;
+        const float big = warp_max(fine ? fabsf(vs) : 0.0f);
+        const uint32_t odd = __ballot_sync(0xffffffffu, !fine);
+        sm->ks[sl][t] = ks * kscale;
+        sm->vs[sl][t] = fine ? vs : 0.0f;
+        if (lane == 0) sm->vmax[sl][t >> 5] = big, sm->odd[sl][t >> 5] = odd;
       }
-      load_scales(regs[u]);
-      advance();
-    }
-    while (ok && ahead > 0) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (ok && ahead > 0) convert(regs[u]);
+      if (++b == end) open();
+      if (!ok) break;
+      if (more) load_scales();
+      convert(2 * gb, T());
+      if (!ready(2 * gb + 1)) break;
+      convert(2 * gb + 1, __half());
+      ++gb;
     }
   } else {
     regs_down<kRegsMma>();
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
       // ---------------- MMA ----------------
       constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
       constexpr uint32_t id_s = umma_idesc_16(fmt, false, kTileRows, kBlock), id_o = umma_idesc_16(0, true, kTileRows, D);
-      auto wait = [&](uint64_t* bar, uint32_t phase) { return mbar_park(bar, phase & 1, st, kStatusTimeout); };
+      auto wait = [&](uint64_t* bar, uint32_t phase) { return mbar_wait_warp(bar, phase & 1, st, kStatusTimeout); };
       auto filled = [&](uint32_t i) { return wait(&sm->full[i % S::kSlots], i / S::kSlots); };
+      // descriptors advance by their address field (in 16 bytes), which never carries out of it
+      const uint64_t q_desc = umma_desc_sw128(smem_addr(smem), 16, 1024);
+      const uint64_t k_desc = umma_desc_sw128(smem_addr(smem + S::kRing), 16, 1024);
+      const uint64_t v_desc = umma_desc_sw128(smem_addr(smem + S::kRing), S::kKvHalf, 1024);
       auto scores = [&](int s, int q_tile, uint32_t i) {
-        const uint32_t q = smem_addr(smem + q_tile * S::kQ), k = smem_addr(slot(i));
         tc_fence_after();
+        if (elect_one()) {
+          const uint64_t q = q_desc + q_tile * (S::kQ >> 4), k = k_desc + (i % S::kSlots) * (S::kKv >> 4);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-          tc_mma_f16_ss(tmem + s * kTmemS, umma_desc_sw128(q + (d / 4) * S::kQHalf + (d % 4) * 32, 16, 1024),
-                        umma_desc_sw128(k + (d / 4) * S::kKvHalf + (d % 4) * 32, 16, 1024), id_s, d > 0);
-        tc_commit(&sm->s_full[s]);
+          for (int d = 0; d < D / 16; ++d)
+            tc_mma_f16_ss(tmem + s * kTmemS, q + (d / 4) * (S::kQHalf >> 4) + (d % 4) * 2,
+                          k + (d / 4) * (S::kKvHalf >> 4) + (d % 4) * 2, id_s, d > 0);
+          tc_commit(&sm->s_full[s]);
+        }
+        __syncwarp();
       };
       auto values = [&](int s, uint32_t i, bool acc) {
-        const uint32_t v = smem_addr(slot(i));
         tc_fence_after();
+        if (elect_one()) {
+          const uint64_t v = v_desc + (i % S::kSlots) * (S::kKv >> 4);
 #pragma unroll
-        for (int k = 0; k < kBlock / 16; ++k)
-          tc_mma_f16_ts(tmem + kTmemO + s * D, tmem + s * kTmemS + 8 * k, umma_desc_sw128(v + 2048 * k, S::kKvHalf, 1024),
-                        id_o, acc || k > 0);
-        tc_commit(&sm->pv_done[s]);
+          for (int k = 0; k < kBlock / 16; ++k)
+            tc_mma_f16_ts(tmem + kTmemO + s * D, tmem + s * kTmemS + 8 * k, v + 128 * k, id_o, acc || k > 0);
+          tc_commit(&sm->pv_done[s]);
+        }
+        __syncwarp();
       };
-      auto release = [&](uint32_t i) { tc_commit(&sm->empty[i % S::kSlots]); };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      auto release = [&](uint32_t i) { commit(&sm->empty[i % S::kSlots]); };
       uint32_t gb = 0, done[2] = {0, 0};
       bool ok = true;
       for (uint32_t part = 0;; ++part) {
@@ -769,7 +774,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         const int nb = sm->part[part % kParts].nb;
         const bool dual = sm->part[part % kParts].dual;
         if (nb == 0) break;
-        give_back(part);
+        __syncwarp();
+        if (lane == 0) give_back(part);
         const uint32_t i0 = 2 * gb;  // ring index of block j's K: i0 + 2 j, of its V: one more
         ok = wait(&sm->q_full, part) && filled(i0);
         if (!ok) break;
@@ -777,7 +783,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
           scores(0, 0, i0);
           scores(1, 1, i0);
           release(i0);
-          if (nb == 1) tc_commit(&sm->q_empty);
+          if (nb == 1) commit(&sm->q_empty);
           for (int j = 0; j < nb && ok; ++j) {
             const uint32_t vi = i0 + 2 * j + 1, kn = vi + 1;
             const bool again = j + 1 < nb;
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             if (!ok) break;
             release(vi);
             if (again) release(kn);
-            if (j + 2 == nb) tc_commit(&sm->q_empty);
+            if (j + 2 == nb) commit(&sm->q_empty);
           }
         } else {
           scores(0, 0, i0);
@@ -803,7 +809,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             scores(1, 0, i0 + 2);
             release(i0 + 2);
           }
-          if (nb <= 2) tc_commit(&sm->q_empty);
+          if (nb <= 2) commit(&sm->q_empty);
           for (int j = 0; j < nb && ok; ++j) {
             const int s = j & 1;
             const uint32_t vi = i0 + 2 * j + 1, kn = vi + 3;
@@ -817,7 +823,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
               if (!ok) break;
               scores(s, 0, kn);
               release(kn);
-              if (j + 3 == nb) tc_commit(&sm->q_empty);
+              if (j + 3 == nb) commit(&sm->q_empty);
             }
           }
         }
@@ -825,31 +831,53 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         gb += nb;
       }
       if (!ok) {  // let what was issued end before TMEM and shared memory go
-        tc_commit(&sm->q_empty);
-        mbar_park(&sm->q_empty, 0, nullptr, 0);
-        mbar_park(&sm->q_empty, 1, nullptr, 0);
+        commit(&sm->q_empty);
+        mbar_wait(&sm->q_empty, 0, nullptr, 0);
+        mbar_wait(&sm->q_empty, 1, nullptr, 0);
       }
     } else if (warp == 13) {
       // ---------------- parts ----------------
+      // and the loads of their K and V rows: a block's rows of a head are one piece of memory
       Walk walk;
       Part p = walk.begin(a, w, blockIdx.x, G, lane);
-      for (uint32_t i = 0;; ++i) {
-        if (i >= kParts && !mbar_park_warp(&sm->part_empty[i % kParts], (i / kParts - 1) & 1, st, kStatusTimeout)) break;
+      uint32_t tile = 0;
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        if (i >= kParts)
+          ok = mbar_wait_warp_sleep(&sm->part_empty[i % kParts], (i / kParts - 1) & 1, st, kStatusTimeout, 100);
+        if (!ok) break;
         if (lane == 0) {
           sm->part[i % kParts] = p;
           mbar_arrive(&sm->part_full[i % kParts]);
         }
         __syncwarp();
         if (p.nb == 0) break;
+        for (int b = p.b0; b < p.b0 + p.nb && ok; ++b) {
+          const uint32_t bytes = static_cast<uint32_t>(min(kBlock, p.len - b * kBlock)) * D;
+          const int64_t at = (p.key0 + static_cast<int64_t>(b) * kBlock) * D;
+          for (int v = 0; v < 2 && ok; ++v, ++tile) {
+            const uint32_t r = tile % S::kRaws;
+            if (tile >= S::kRaws)
+              ok = mbar_wait_warp_sleep(&sm->raw_empty[r], (tile / S::kRaws - 1) & 1, st, kStatusTimeout, 40);
+            if (ok && lane == 0) {
+              mbar_arrive_expect_tx(&sm->raw_full[r], bytes);
+              bulk_g2s(smem + S::kRaw + r * S::kRawTile, (v ? a.v : a.k) + at, bytes, &sm->raw_full[r]);
+            }
+            __syncwarp();
+          }
+        }
         p = walk.next(a, w, blockIdx.x, G);
       }
+      // every copy has landed before the block's shared memory goes
+      for (uint32_t i = tile > S::kRaws ? tile - S::kRaws : 0; i < tile; ++i)
+        mbar_wait_warp(&sm->raw_full[i % S::kRaws], (i / S::kRaws) & 1, st, kStatusTimeout);
     } else if (warp > 13) {
       // ---------------- Q ----------------
       bool ok = true;
       for (uint32_t part = 0;; ++part) {
         const Part& pt = take(part, ok);
         if (!ok || pt.nb == 0) break;
-        if (part > 0) ok = mbar_park_warp(&sm->q_empty, (part - 1) & 1, st, kStatusTimeout);
+        if (part > 0) ok = mbar_wait_warp_sleep(&sm->q_empty, (part - 1) & 1, st, kStatusTimeout, 100);
         if (!ok) break;
         const int rows = pt.nt * G, first = pt.dual ? half * G : rows, tiles = pt.dual ? 2 : 1;
         const T* q0 = static_cast<const T*>(a.q) + static_cast<int64_t>(pt.t0) * a.q_ld + static_cast<int64_t>(pt.kv) * G * D;
@@ -925,7 +953,7 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
       const float top = fmaxf(m, warp_max(ml.x));
       const float old = m == -INFINITY ? 0.0f : ex2_approx(m - top);
       const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ex2_approx(ml.x - top);
-      l = l * old + warp_sum(f == 0.0f ? 0.0f : f * ml.y);
+      l = l * old + warp_sum(f == 0.0f && ml.y == ml.y ? 0.0f : f * ml.y);
       m = top;
 #pragma unroll
       for (int e = 0; e < N; ++e) o[e] *= old;
