@@ -39,7 +39,6 @@ namespace {
 
 constexpr int kTileRows = 128;     // of a stream
 constexpr int kBlock = 96;         // keys: three pairs of K and V tiles and both Q tiles fill the shared memory
-constexpr int kMinPiece = 2;       // places of the line in a CTA's piece; even, see Tile
 constexpr int kPlanThreads = 1024;
 constexpr int kAttendThreads = 512;  // warpgroups: softmax of stream 0, of stream 1, conversion, MMA and Q
 constexpr int kRegsSoftmax = 176, kRegsConvert = 80, kRegsMma = 80;  // 2 x 176 + 80 + 80 = 4 x the 128 of the launch
@@ -47,8 +46,10 @@ constexpr float kRaiseMax = 8.0f;   // a row's reference is raised when it is to
 constexpr float kHeadroom = 6.0f;   // of it below the largest weight x scale
 constexpr int kLeastExp = -40;      // of a block's largest V scale: blocks of zeros must not push the sums out of range
 
-// Tokens and keys of a unit (with a KV head). A block takes two places of the line when both streams work on it and one
-// otherwise (rounded up to an even count), so places measure time and an even cut never divides a block.
+// Tokens and keys of a unit (with a KV head). Its places on the line: one for each block (a block takes about as long for
+// 256 rows as for 128: 3900 and 3700 cycles), after `open` for what a part costs before its first block and after its last.
+// Batches of fewer than kFewBlocks blocks a CTA are cut into single blocks instead (open 0).
+constexpr int kOpen = 2, kFewBlocks = 4;
 struct Tile {
   int32_t t0, nt;      // tokens
   int32_t base, len;   // key rows
@@ -60,8 +61,9 @@ struct Tile {
 };
 struct PlanHead {
   int32_t tiles;
-  int32_t per;       // places of a piece, even
+  int32_t per;       // places of a piece, more than open
   int64_t total;     // places of all units
+  int32_t open;
 };
 
 struct SharedWs {  // the workspace's parts
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
   if (n_tiles > w.prefix_tiles) {  // groups that overlap one another: no result
     for (int t = tid; t < a.n; t += kPlanThreads) w.tok_own[t] = -1;
     if (tid == 0) {
-      *w.head = PlanHead{0, 1, 0};
+      *w.head = PlanHead{0, 1, 0, 0};
       if (a.status) atomicCAS(a.status, 0, kStatusBadIndex);
     }
     return;
@@ -252,36 +254,48 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
   }
   __syncthreads();
   // places before each tile, then the pieces' length, then partial rows before each tile
-  int64_t places = 0;
+  int64_t places = 0, n_units = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int64_t mine = 0;
+    int64_t mine = 0, units = 0;
     if (i < n_tiles) {
       Tile& x = w.tile[i];
       if (i >= own0) x.nt = w.tile[i + 1].t0 - x.t0;
       x.blocks = (x.len + kBlock - 1) / kBlock;
       x.dual = x.nt > half;
-      x.places = x.dual ? 2 * x.blocks : (x.blocks + 1) / 2 * 2;
-      mine = static_cast<int64_t>(x.places) * a.KV;
+      mine = static_cast<int64_t>(x.blocks) * a.KV;
+      units = x.blocks > 0 ? a.KV : 0;
     }
     int64_t total;
     const int64_t incl = block_scan_sum(mine, part64, total);
-    if (i < n_tiles) w.tile[i].first = places + incl - mine;
+    int64_t opened;
+    const int64_t before = block_scan_sum(units, part64, opened);
+    if (i < n_tiles) {
+      w.tile[i].first = places + incl - mine;
+      w.tile[i].row = n_units + before - units;
+    }
     places += total;
+    n_units += opened;
   }
-  const int per = static_cast<int>(max(static_cast<int64_t>(kMinPiece), (places + 2 * ctas - 1) / (2 * ctas) * 2));
+  const int open = places < static_cast<int64_t>(kFewBlocks) * ctas ? 0 : kOpen;
+  places += open * n_units;
+  const int per = static_cast<int>(max(static_cast<int64_t>(open + 1), (places + ctas - 1) / ctas));
   int64_t rows = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int64_t mine = 0;
-    if (i < n_tiles && w.tile[i].blocks > 0)
-      mine = pieces_bound(w.tile[i].places, per) * a.KV * w.tile[i].nt * G;
+    if (i < n_tiles) {
+      Tile& x = w.tile[i];
+      x.first += open * x.row;
+      x.places = x.blocks > 0 ? open + x.blocks : 0;
+      if (x.blocks > 0) mine = pieces_bound(x.places, per) * a.KV * x.nt * G;
+    }
     int64_t total;
     const int64_t incl = block_scan_sum(mine, part64, total);
     if (i < n_tiles) w.tile[i].row = rows + incl - mine;
     rows += total;
   }
-  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows ? places : 0};
+  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows ? places : 0, open};
   if (bad && a.status) atomicCAS(a.status, 0, kStatusBadIndex);
 }
 
@@ -300,24 +314,40 @@ struct Part {
 struct Walk {
   int done, tile, kv, span;  // places before the current part, its unit and its places
 
-  // The part that begins at `done` (nb 0: none).
+  // The first part with blocks at or behind `done` (nb 0: none).
   __device__ __forceinline__ Part part(const SharedArgs& a, const SharedWs& w, int cta, int G) {
     Part p{};
     const PlanHead h = *w.head;
-    const int64_t from = static_cast<int64_t>(cta) * h.per, at = from + done, end = min(h.total, from + h.per);
-    if (at >= end || tile >= h.tiles) return p;
-    const Tile x = w.tile[tile];
-    const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
-    const int p0 = static_cast<int>(at - first);
-    const int p1 = static_cast<int>(min(static_cast<int64_t>(x.places), p0 + (end - at)));
-    span = p1 - p0;
-    p.b0 = x.dual ? p0 / 2 : p0;
-    p.nb = (x.dual ? p1 / 2 : min(p1, x.blocks)) - p.b0;
-    p.t0 = x.t0, p.nt = x.nt, p.len = x.len, p.kv = kv;
-    p.own = x.own != 0, p.dual = x.dual != 0;
-    p.key0 = static_cast<int64_t>(kv) * a.n_rows + x.base;
-    p.row = x.row + (kv * pieces_bound(x.places, h.per) + (at / h.per - first / h.per)) * x.nt * G;
+    const int64_t from = static_cast<int64_t>(cta) * h.per, end = min(h.total, from + h.per);
+    while (from + done < end && tile < h.tiles) {
+      const int64_t at = from + done;
+      const Tile x = w.tile[tile];
+      const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
+      const int p0 = static_cast<int>(at - first);
+      const int p1 = static_cast<int>(min(static_cast<int64_t>(x.places), p0 + (end - at)));
+      span = p1 - p0;
+      p.b0 = max(0, p0 - h.open);
+      p.nb = max(0, p1 - h.open) - p.b0;
+      if (p.nb > 0) {
+        p.t0 = x.t0, p.nt = x.nt, p.len = x.len, p.kv = kv;
+        p.own = x.own != 0, p.dual = x.dual != 0;
+        p.key0 = static_cast<int64_t>(kv) * a.n_rows + x.base;
+        p.row = x.row + (kv * pieces_bound(x.places, h.per) + (at / h.per - first / h.per)) * x.nt * G;
+        return p;
+      }
+      step(a, w);
+    }
+    p.nb = 0;
     return p;
+  }
+  __device__ __forceinline__ void step(const SharedArgs& a, const SharedWs& w) {
+    done += span;
+    if (++kv == a.KV) {
+      kv = 0;
+      ++tile;
+      const int tiles = w.head->tiles;
+      while (tile < tiles && w.tile[tile].blocks == 0) ++tile;
+    }
   }
   // One whole warp calls it.
   __device__ __forceinline__ Part begin(const SharedArgs& a, const SharedWs& w, int cta, int G, int lane) {
@@ -339,13 +369,7 @@ struct Walk {
     return part(a, w, cta, G);
   }
   __device__ __forceinline__ Part next(const SharedArgs& a, const SharedWs& w, int cta, int G) {
-    done += span;
-    if (++kv == a.KV) {
-      kv = 0;
-      ++tile;
-      const int tiles = w.head->tiles;
-      while (tile < tiles && w.tile[tile].blocks == 0) ++tile;
-    }
+    step(a, w);
     return part(a, w, cta, G);
   }
 };
@@ -394,7 +418,7 @@ constexpr int kScaleSlots = 4;  // a block's scales are overwritten four blocks 
 constexpr int kParts = 4;       // parts known ahead
 struct SharedSmall {
   uint64_t part_full[kParts], part_empty[kParts];
-  uint64_t q_full, q_empty, full[5], empty[5], raw_full[3], raw_empty[3], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
+  uint64_t q_full[2], q_empty[2], full[5], empty[5], raw_full[3], raw_empty[3], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
   alignas(16) float ks[kScaleSlots][kBlock];  // K scale x scale x log2 e
   alignas(16) float vs[kScaleSlots][kBlock];
   alignas(16) float vmax[kScaleSlots][4];     // largest finite |V scale| of each 32 keys of the block
@@ -427,12 +451,10 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
   }
   if (warp == 12) tmem_alloc(&sm->tmem, 512);
   if (threadIdx.x == 0) {
-    mbar_init(&sm->q_full, 64);
     for (int i = 0; i < kParts; ++i) {
       mbar_init(&sm->part_full[i], 1);
       mbar_init(&sm->part_empty[i], 15);  // 8 softmax, 4 conversion and 2 Q warps, the MMA warp
     }
-    mbar_init(&sm->q_empty, 1);
     mbar_init(&sm->b_fin, 4);
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(&sm->full[i], 128);
@@ -443,6 +465,8 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       mbar_init(&sm->raw_empty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm->q_full[i], 64);
+      mbar_init(&sm->q_empty[i], 1);
       mbar_init(&sm->s_full[i], 1);
       mbar_init(&sm->p_full[i], 4);
       mbar_init(&sm->pv_done[i], 1);
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       const bool dual = pt.dual;
       const int rows = (dual ? (s ? pt.nt - half : half) : pt.nt) * G;
       const bool on = (warp & 3) * 32 < rows;
-      int limit = 0;  // keys this row sees
+      int limit = pt.len;  // keys this row sees (a row without a token may see all: what comes of it is not looked at)
       if (row < rows) limit = pt.own ? own_keys(a, pt.t0 + (dual && s ? half : 0) + row / G, nullptr) : pt.len;
       limit -= pt.b0 * kBlock;
       float m = -INFINITY, l = 0.0f;
@@ -777,13 +801,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         __syncwarp();
         if (lane == 0) give_back(part);
         const uint32_t i0 = 2 * gb;  // ring index of block j's K: i0 + 2 j, of its V: one more
-        ok = wait(&sm->q_full, part) && filled(i0);
+        // a part whose streams share their rows has them in one of the two Q tiles, in turn, so that the next part's can come in
+        const int qt = part & 1;
+        auto q_done = [&]() {
+          if (dual || qt == 0) commit(&sm->q_empty[0]);
+          if (dual || qt == 1) commit(&sm->q_empty[1]);
+        };
+        ok = wait(&sm->q_full[part & 1], part >> 1) && filled(i0);
         if (!ok) break;
         if (dual) {
           scores(0, 0, i0);
           scores(1, 1, i0);
           release(i0);
-          if (nb == 1) commit(&sm->q_empty);
+          if (nb == 1) q_done();
           for (int j = 0; j < nb && ok; ++j) {
             const uint32_t vi = i0 + 2 * j + 1, kn = vi + 1;
             const bool again = j + 1 < nb;
@@ -798,18 +828,18 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             if (!ok) break;
             release(vi);
             if (again) release(kn);
-            if (j + 2 == nb) commit(&sm->q_empty);
+            if (j + 2 == nb) q_done();
           }
         } else {
-          scores(0, 0, i0);
+          scores(0, qt, i0);
           release(i0);
           if (nb > 1) {
             ok = filled(i0 + 2);
             if (!ok) break;
-            scores(1, 0, i0 + 2);
+            scores(1, qt, i0 + 2);
             release(i0 + 2);
           }
-          if (nb <= 2) commit(&sm->q_empty);
+          if (nb <= 2) q_done();
           for (int j = 0; j < nb && ok; ++j) {
             const int s = j & 1;
             const uint32_t vi = i0 + 2 * j + 1, kn = vi + 3;
@@ -821,9 +851,9 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             if (j + 2 < nb) {
               ok = filled(kn);
               if (!ok) break;
-              scores(s, 0, kn);
+              scores(s, qt, kn);
               release(kn);
-              if (j + 3 == nb) commit(&sm->q_empty);
+              if (j + 3 == nb) q_done();
             }
           }
         }
@@ -831,9 +861,9 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         gb += nb;
       }
       if (!ok) {  // let what was issued end before TMEM and shared memory go
-        commit(&sm->q_empty);
-        mbar_wait(&sm->q_empty, 0, nullptr, 0);
-        mbar_wait(&sm->q_empty, 1, nullptr, 0);
+        commit(&sm->q_empty[0]);
+        mbar_wait(&sm->q_empty[0], 0, nullptr, 0);
+        mbar_wait(&sm->q_empty[0], 1, nullptr, 0);
       }
     } else if (warp == 13) {
       // ---------------- parts ----------------
@@ -873,28 +903,33 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
         mbar_wait_warp(&sm->raw_full[i % S::kRaws], (i / S::kRaws) & 1, st, kStatusTimeout);
     } else if (warp > 13) {
       // ---------------- Q ----------------
+      // rows without a token keep what is there: what comes of them is not looked at
       bool ok = true;
+      uint32_t uses[2] = {0, 0};  // parts that used each of the two tiles
       for (uint32_t part = 0;; ++part) {
         const Part& pt = take(part, ok);
         if (!ok || pt.nb == 0) break;
-        if (part > 0) ok = mbar_wait_warp_sleep(&sm->q_empty, (part - 1) & 1, st, kStatusTimeout, 100);
+        const bool dual = pt.dual;
+#pragma unroll
+        for (uint32_t q = 0; q < 2; ++q) {
+          if (!ok || !(dual || (part & 1) == q)) continue;
+          if (uses[q] > 0) ok = mbar_wait_warp_sleep(&sm->q_empty[q], (uses[q] - 1) & 1, st, kStatusTimeout, 40);
+          ++uses[q];
+        }
         if (!ok) break;
-        const int rows = pt.nt * G, first = pt.dual ? half * G : rows, tiles = pt.dual ? 2 : 1;
+        const int rows = pt.nt * G, first = dual ? half * G : rows;
         const T* q0 = static_cast<const T*>(a.q) + static_cast<int64_t>(pt.t0) * a.q_ld + static_cast<int64_t>(pt.kv) * G * D;
-        for (int i = threadIdx.x - 448; i < tiles * kTileRows * (D / 8); i += 64) {
-          const int r = i / (D / 8), c = i % (D / 8), tile = r / kTileRows, q = r % kTileRows;
-          uint8_t* dst = smem + tile * S::kQ + (c / 8) * S::kQHalf + q * 128 + (((c % 8) ^ (q & 7)) * 16);
-          if (q < (tile ? rows - first : first)) {
-            const int at = tile * first + q;
-            cp_async16(dst, q0 + static_cast<int64_t>(at / G) * a.q_ld + static_cast<int64_t>(at % G) * D + 8 * c);
-          } else {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);  // rows without a token
-          }
+#pragma unroll 4
+        for (int i = threadIdx.x - 448; i < rows * (D / 8); i += 64) {
+          const int at = i / (D / 8), c = i % (D / 8), second = at >= first ? 1 : 0, q = at - second * first;
+          uint8_t* tile = smem + (dual ? second : static_cast<int>(part & 1)) * S::kQ;
+          cp_async16(tile + (c / 8) * S::kQHalf + q * 128 + (((c % 8) ^ (q & 7)) * 16),
+                     q0 + static_cast<int64_t>(at / G) * a.q_ld + static_cast<int64_t>(at % G) * D + 8 * c);
         }
         cp_async_commit();
         cp_async_wait<0>();
         fence_async_smem();
-        mbar_arrive(&sm->q_full);
+        mbar_arrive(&sm->q_full[part & 1]);
         __syncwarp();
         if (lane == 0) give_back(part);
       }
@@ -941,6 +976,7 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
       n[which] = static_cast<int>((first + x.places - 1) / head.per - first / head.per) + 1;
       dist[which] = static_cast<int64_t>(x.nt) * G;
       r0[which] = x.row + kv * pieces_bound(x.places, head.per) * dist[which] + (t - x.t0) * G + h % G;
+      if ((first / head.per + 1) * head.per - first <= head.open) --n[which], r0[which] += dist[which];  // cut before its blocks
     }
     for (int p0 = 0; p0 < n[0] + n[1]; p0 += 32) {  // a lane per piece, then the pieces' rows, four at a time
       const int p = p0 + lane, all = min(32, n[0] + n[1] - p0);
