@@ -19,6 +19,7 @@
 // down to 2^-20 of the largest. Sums and outputs carry the same reference, so it cancels.
 // Bound: HBM for one tile of rows a group (128 rows: 65.5 kFLOP against 264 bytes a key and head, the machine's balance),
 // the tensor pipe and the conversion above that.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -31,6 +32,7 @@
 #include "kernels.hpp"
 #include "pdl.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.hpp"
 #include "types16.cuh"
 
 namespace mkb {
@@ -312,16 +314,16 @@ struct Part {
 };
 
 struct Walk {
+  PlanHead h;
+  Tile x;                    // the current tile
   int done, tile, kv, span;  // places before the current part, its unit and its places
 
   // The first part with blocks at or behind `done` (nb 0: none).
   __device__ __forceinline__ Part part(const SharedArgs& a, const SharedWs& w, int cta, int G) {
     Part p{};
-    const PlanHead h = *w.head;
     const int64_t from = static_cast<int64_t>(cta) * h.per, end = min(h.total, from + h.per);
     while (from + done < end && tile < h.tiles) {
       const int64_t at = from + done;
-      const Tile x = w.tile[tile];
       const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
       const int p0 = static_cast<int>(at - first);
       const int p1 = static_cast<int>(min(static_cast<int64_t>(x.places), p0 + (end - at)));
@@ -344,14 +346,15 @@ struct Walk {
     done += span;
     if (++kv == a.KV) {
       kv = 0;
-      ++tile;
-      const int tiles = w.head->tiles;
-      while (tile < tiles && w.tile[tile].blocks == 0) ++tile;
+      while (++tile < h.tiles) {
+        x = w.tile[tile];
+        if (x.blocks > 0) break;
+      }
     }
   }
   // One whole warp calls it.
   __device__ __forceinline__ Part begin(const SharedArgs& a, const SharedWs& w, int cta, int G, int lane) {
-    const PlanHead h = *w.head;
+    h = *w.head;
     const int64_t at = static_cast<int64_t>(cta) * h.per;
     // the last tile that begins at or before `at`: 32 probes a round
     int lo = 0, hi = h.tiles;
@@ -365,7 +368,8 @@ struct Walk {
     }
     done = 0;
     tile = lo;
-    kv = static_cast<int>((at - w.tile[lo].first) / w.tile[lo].places);
+    x = w.tile[lo];
+    kv = static_cast<int>((at - x.first) / x.places);
     return part(a, w, cta, G);
   }
   __device__ __forceinline__ Part next(const SharedArgs& a, const SharedWs& w, int cta, int G) {
@@ -437,8 +441,16 @@ constexpr int shared_smem() {
 }
 constexpr uint32_t kTmemS = 128, kTmemO = 256;  // columns: S0 | S1 at 0 and 128, O0 | O1 from 256
 
+// A lane's 32 bytes as one whole sector: a lane has a row of its own, so halves would be two requests each.
+__device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs a, SharedWs w) {
+__global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(const __grid_constant__ CUtensorMap mq,
+                                                                     SharedArgs a, SharedWs w) {
   using S = SharedShape<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   SharedSmall* sm = reinterpret_cast<SharedSmall*>(smem + S::kSmall);
@@ -453,7 +465,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kParts; ++i) {
       mbar_init(&sm->part_full[i], 1);
-      mbar_init(&sm->part_empty[i], 15);  // 8 softmax, 4 conversion and 2 Q warps, the MMA warp
+      mbar_init(&sm->part_empty[i], 14);  // 8 softmax and 4 conversion warps, the MMA and the Q warp
     }
     mbar_init(&sm->b_fin, 4);
     for (int i = 0; i < S::kSlots; ++i) {
@@ -465,7 +477,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       mbar_init(&sm->raw_empty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm->q_full[i], 64);
+      mbar_init(&sm->q_full[i], 1);
       mbar_init(&sm->q_empty[i], 1);
       mbar_init(&sm->s_full[i], 1);
       mbar_init(&sm->p_full[i], 4);
@@ -652,8 +664,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
             }
             if (row < rows) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4*>(o + 32 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+              for (int i = 0; i < 32; i += 8) store_sector(o + 32 * c + i, v + i);
             }
             __syncwarp();
           }
@@ -901,11 +912,13 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
       // every copy has landed before the block's shared memory goes
       for (uint32_t i = tile > S::kRaws ? tile - S::kRaws : 0; i < tile; ++i)
         mbar_wait_warp(&sm->raw_full[i % S::kRaws], (i / S::kRaws) & 1, st, kStatusTimeout);
-    } else if (warp > 13) {
+    } else if (warp == 14) {
       // ---------------- Q ----------------
-      // rows without a token keep what is there: what comes of them is not looked at
+      // rows are (token, query head of the KV head), so 64 columns of a tile are one box of the tensor; behind a part's last
+      // token it holds others', and what comes of those is not looked at
       bool ok = true;
       uint32_t uses[2] = {0, 0};  // parts that used each of the two tiles
+      uint32_t issued = 0;
       for (uint32_t part = 0;; ++part) {
         const Part& pt = take(part, ok);
         if (!ok || pt.nb == 0) break;
@@ -917,22 +930,24 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(SharedArgs 
           ++uses[q];
         }
         if (!ok) break;
-        const int rows = pt.nt * G, first = dual ? half * G : rows;
-        const T* q0 = static_cast<const T*>(a.q) + static_cast<int64_t>(pt.t0) * a.q_ld + static_cast<int64_t>(pt.kv) * G * D;
-#pragma unroll 4
-        for (int i = threadIdx.x - 448; i < rows * (D / 8); i += 64) {
-          const int at = i / (D / 8), c = i % (D / 8), second = at >= first ? 1 : 0, q = at - second * first;
-          uint8_t* tile = smem + (dual ? second : static_cast<int>(part & 1)) * S::kQ;
-          cp_async16(tile + (c / 8) * S::kQHalf + q * 128 + (((c % 8) ^ (q & 7)) * 16),
-                     q0 + static_cast<int64_t>(at / G) * a.q_ld + static_cast<int64_t>(at % G) * D + 8 * c);
+        if (lane == 0) {
+          uint64_t* bar = &sm->q_full[part & 1];
+          const int tiles = dual ? 2 : 1;
+          mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles * S::kHalves * half * G * 128));
+          for (int q = 0; q < tiles; ++q)
+#pragma unroll
+            for (int x = 0; x < S::kHalves; ++x)
+              tma_load_3d(smem + (dual ? q : static_cast<int>(part & 1)) * S::kQ + x * S::kQHalf, &mq, 64 * x, pt.kv * G,
+                          pt.t0 + q * half, bar);
+          issued = part + 1;
         }
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_async_smem();
-        mbar_arrive(&sm->q_full[part & 1]);
         __syncwarp();
         if (lane == 0) give_back(part);
       }
+      // every copy has landed before the block's shared memory goes
+      if (lane == 0)
+        for (uint32_t i = issued > 2 ? issued - 2 : 0; i < issued; ++i)
+          mbar_wait(&sm->q_full[i & 1], (i >> 1) & 1, st, kStatusTimeout);
     }
   }
   __syncwarp();
@@ -952,6 +967,8 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
   if (id >= static_cast<int64_t>(a.n) * a.H) return;
   const int t = static_cast<int>(id / a.H), h = static_cast<int>(id % a.H), G = a.H / a.KV, kv = h / G;
   const PlanHead head = *w.head;
+  const int pre = head.total > 0 ? w.tok_pre[t] : -1, own = head.total > 0 ? w.tok_own[t] : -1;
+  const Tile tiles[2] = {w.tile[max(pre, 0)], w.tile[max(own, 0)]};
   float m = -INFINITY, l = 0.0f, o[N] = {};
   auto values = [&](const float* p, float (&v)[N]) {
     if constexpr (N == 4) {
@@ -968,10 +985,8 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
     int n[2] = {0, 0};
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const int i = which ? w.tok_own[t] : w.tok_pre[t];
-      if (i < 0) continue;
-      const Tile x = w.tile[i];
-      if (x.blocks == 0) continue;
+      const Tile& x = tiles[which];
+      if ((which ? own : pre) < 0 || x.blocks == 0) continue;
       const int64_t first = x.first + static_cast<int64_t>(kv) * x.places;
       n[which] = static_cast<int>((first + x.places - 1) / head.per - first / head.per) + 1;
       dist[which] = static_cast<int64_t>(x.nt) * G;
@@ -1085,6 +1100,10 @@ int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
     if (at.numRegs * 4 < 2 * kRegsSoftmax + kRegsConvert + kRegsMma) return cudaErrorInvalidConfiguration;
     set[dev] = true;
   }
+  CUtensorMap mq;
+  const int G = a.H / a.KV;
+  const int rc = make_map3(&mq, std::is_same<T, __nv_bfloat16>::value, a.q, D, a.H, a.n, a.q_ld, 64, kTileRows / G, G);
+  if (rc != 0) return rc;
   const int ctas = sms;
   const WsLayout y = ws_layout(a.n, a.H, a.KV, D, a.n_groups, ctas);
   uint8_t* p = static_cast<uint8_t*>(ws);
@@ -1097,7 +1116,7 @@ int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
   e = cudaGetLastError();
   if (e == cudaSuccess)
     e = launch_pdl(k_shared_attend<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(kAttendThreads), shared_smem<D>(), s, 1,
-                   a, w);
+                   mq, a, w);
   const int64_t warps = static_cast<int64_t>(a.n) * a.H;
   if (e == cudaSuccess)
     e = launch_pdl(k_shared_join<T, D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, s, 1, a, w);

@@ -7,10 +7,10 @@
 
 namespace mkb {
 
-// 16-bit values [rows][heads][width], rows `ld` values apart, heads `width` apart: boxes of `box_rows` rows of
-// `box_width` values of one head, 128-byte swizzle, zeros outside. base 16-byte aligned, ld % 8 == 0. 0 or a CUDA error.
+// 16-bit values [rows][heads][width], rows `ld` values apart, heads `width` apart: boxes of `box_rows` rows of `box_heads`
+// heads of `box_width` values, 128-byte swizzle, zeros outside. base 16-byte aligned, ld % 8 == 0. 0 or a CUDA error.
 inline int make_map3(CUtensorMap* map, bool bf16, const void* base, int width, int heads, int64_t rows, int64_t ld,
-                     int box_width, int box_rows) {
+                     int box_width, int box_rows, int box_heads = 1) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -26,7 +26,8 @@ inline int make_map3(CUtensorMap* map, bool bf16, const void* base, int width, i
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads),
                               static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(width) * 2, static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_width), 1, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_heads),
+                             static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t step[3] = {1, 1, 1};
   const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                             const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
