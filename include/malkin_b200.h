@@ -378,16 +378,17 @@ int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* d
  * token t attends to rows dev_kv_base[t] .. + dev_n_keys[t] - 1 and to the rows dev_anc[dev_anc_off[t] ..
  * dev_anc_off[t + 1]) relative to dev_kv_base[t] (dev_anc_off NULL: none; n_anc entries). In addition the tokens
  * dev_group_off[g] .. dev_group_off[g + 1] - 1 (n_groups + 1 ascending entries; a token may be in no group) attend to the
- * rows dev_prefix_base[g] .. + dev_prefix_len[g] - 1, read once for up to 128 / (H / KV) of them. All of a token's keys are
+ * rows dev_prefix_base[g] .. + dev_prefix_len[g] - 1, read once for up to 2 (128 / (H / KV)) of them (rounded down inside). All of a token's keys are
  * in one softmax; a token without any gives zeros. Consecutive tokens with the same dev_kv_base share one pass over its
  * rows, so a request's tokens belong next to each other. n_groups = 0 is allowed.
  * dev_q and dev_out: n rows of H x D, q_ld / out_ld apart, type MK_TYPE_F16 or MK_TYPE_BF16; D 64 or 128, H / KV at most
- * 128, scale > 0; dev_q, dev_k, dev_v, dev_out and dev_ws 16-byte aligned, strides multiples of 8.
+ * 128, scale > 0; dev_q, dev_k, dev_v and dev_out 16-byte aligned, dev_ws 32-byte, strides multiples of 8. A scale of V that
+ * is not finite makes the outputs of the tokens that see its row NaN.
  * Rows outside the tables are not looked at, nor are their scales. A group or token whose rows leave the cache, or a group
  * whose tokens leave 0 .. n, has none of those keys, a token whose ancestors do loses them from the first such one on, and
  * MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside a kernel ran out, the outputs are not valid.
- * dev_ws: mk_attention_shared_workspace(n, H, KV, D, n_groups) bytes (negative: bad shape or no device; about
- * 16 n H (D + 2) bytes and 256 x 128 x (D + 2) x 4 for the largest device). */
+ * dev_ws: mk_attention_shared_workspace(n, H, KV, D, n_groups) bytes (negative: bad shape or no device): the
+ * partial results, 4 (D + 2) bytes for each of 4 n H rows and of 256 rows a multiprocessor, and the tables of the plan. */
 int64_t mk_attention_shared_workspace(int n, int H, int KV, int D, int n_groups);
 int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H, int KV, int D, float scale,
                         const int8_t* dev_k, const int8_t* dev_v, const float* dev_ks, const float* dev_vs,

@@ -601,7 +601,7 @@ int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int
                {dev_status, 4, "dev_status", true}}, who);
     mkb::NormRopeArgs a{dev_qkv, ld, n, H, KV, dev_q_norm, dev_k_norm, eps, dev_rope, n_pos, dev_pos, dev_q, q_ld,
                         dev_k, k_ld, dev_kc, dev_vc, dev_ks, dev_vs, n_rows, dev_kv_at, dev_status};
-    mkb::launch_qk_norm_rope(a, t, D, current_sms(), as_stream(stream));
+    mkb::launch_qk_norm_rope(a, t, D, as_stream(stream));
     mkb::cuda_check(cudaGetLastError(), who);
   });
 }
@@ -660,7 +660,7 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
                {dev_vs, 4, "dev_vs"}, {dev_group_off, 4, "dev_group_off", n_groups == 0},
                {dev_prefix_base, 4, "dev_prefix_base", n_groups == 0}, {dev_prefix_len, 4, "dev_prefix_len", n_groups == 0},
                {dev_kv_base, 4, "dev_kv_base"}, {dev_n_keys, 4, "dev_n_keys"}, {dev_anc_off, 4, "dev_anc_off", true},
-               {anc ? dev_anc : nullptr, 4, "dev_anc", !anc}, {dev_out, 16, "dev_out"}, {dev_ws, 16, "dev_ws"},
+               {anc ? dev_anc : nullptr, 4, "dev_anc", !anc}, {dev_out, 16, "dev_out"}, {dev_ws, 32, "dev_ws"},
                {dev_status, 4, "dev_status", true}}, who);
     const int sms = current_sms();
     if (ws_bytes < mkb::attention_shared_workspace(n, H, KV, D, n_groups, sms))

@@ -40,7 +40,7 @@ namespace mkb {
 namespace {
 
 constexpr int kTileRows = 128;     // of a stream
-constexpr int kBlock = 96;         // keys: three pairs of K and V tiles and both Q tiles fill the shared memory
+constexpr int kBlock = 96;         // keys: five 16-bit K / V tiles, three int8 ones and both Q tiles fill the shared memory
 constexpr int kPlanThreads = 1024;
 constexpr int kAttendThreads = 512;  // warpgroups: softmax of stream 0, of stream 1, conversion, MMA and Q
 constexpr int kRegsSoftmax = 176, kRegsConvert = 80, kRegsMma = 80;  // 2 x 176 + 80 + 80 = 4 x the 128 of the launch
@@ -441,7 +441,7 @@ constexpr int shared_smem() {
 }
 constexpr uint32_t kTmemS = 128, kTmemO = 256;  // columns: S0 | S1 at 0 and 128, O0 | O1 from 256
 
-// A lane's 32 bytes as one whole sector: a lane has a row of its own, so halves would be two requests each.
+// A lane's 32 bytes as one whole sector (p 32-byte aligned): a lane has a row of its own, so halves would be two requests each.
 __device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])

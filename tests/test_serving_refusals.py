@@ -62,7 +62,7 @@ def shared(mk, **k):
     dict(type_=F32), dict(H=5), dict(H=0), dict(D=80), dict(n=-1), dict(n_groups=-1), dict(n_rows=0), dict(n_anc=-1),
     dict(H=258, KV=2, q_ld=258 * 128, out_ld=258 * 128), dict(scale=0.0), dict(scale=float("nan")), dict(q_ld=508),
     dict(q_ld=515), dict(out_ld=511), dict(dev_q=P + 8), dict(dev_k=P + 4), dict(dev_out=P + 4), dict(dev_ws=P + 8),
-    dict(dev_ks=0), dict(dev_group_off=0), dict(dev_kv_base=0), dict(dev_n_keys=P + 1), dict(dev_anc=0)])
+    dict(dev_ws=P + 16), dict(dev_ks=0), dict(dev_group_off=0), dict(dev_kv_base=0), dict(dev_n_keys=P + 1), dict(dev_anc=0)])
 def test_shared_refuses(mk, change):
     refused(mk, shared, mk, **change)
 
