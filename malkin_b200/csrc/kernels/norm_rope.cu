@@ -7,7 +7,11 @@
 // q = round(y / d), taken from the fp32 values, not from the rounded 16-bit ones.
 //
 // Bound: memory. A group of D / 8 lanes owns one head, each lane four values of the first half and the four they pair
-// with, so the rotation needs no exchange and both halves are loaded and stored as whole 8- or 16-byte words.
+// with, so the rotation needs no exchange and both halves are loaded and stored as whole 8- or 16-byte words. The head's
+// values and the weights are asked for before the first of them is used. At 16384 tokens of 32 + 8 + 8 heads of 128 in bf16
+// with their cache rows it takes 104 to 115 us (3.5 to 3.9 TB/s), on fp32 rows without a cache (8192 tokens, 40 heads) 56 to
+// 65 (5.2 to 6.0 TB/s). Eight values a lane (16-byte words of 16-bit types) take 109 there and 61; two, three and four heads a
+// lane one after the other 125, 104 and 123; a token's heads in rounds, angles and weights kept in registers, 112.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -70,15 +74,26 @@ __device__ __forceinline__ void store_i8x4(int8_t* p, const float (&v)[4], float
   *reinterpret_cast<uint32_t*>(p) = w;
 }
 
-// Grid: (token, head slice). A group takes heads g, g + groups, ... of its slice.
+// Grid: (token, its heads by the block's groups). A block past the last head's group has lanes without a head; they run
+// along, so that the shuffles see whole warps.
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(kNrThreads)
-    k_qk_norm_rope(NormRopeArgs a) {
+__global__ void __launch_bounds__(kNrThreads) k_qk_norm_rope(NormRopeArgs a) {
   constexpr int LANES = D / 8, GROUPS = kNrThreads / LANES, HALF = D / 2;
-  const int t = blockIdx.x, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int heads = a.H + a.KV + (a.kc ? a.KV : 0);
+  const int t = blockIdx.x, lane = threadIdx.x % LANES, i0 = 4 * lane;
+  const int h = blockIdx.y * GROUPS + threadIdx.x / LANES;
+  const bool on = h < a.H + a.KV + (a.kc ? a.KV : 0), rotated = h < a.H + a.KV;
   const int pos = a.pos[t];
-  const bool in_table = pos >= 0 && pos < a.n_pos;
+  float x0[4] = {}, x1[4] = {}, w0[4] = {}, w1[4] = {};
+  if (on) {
+    const T* x = static_cast<const T*>(a.qkv) + static_cast<int64_t>(t) * a.ld + static_cast<int64_t>(h) * D + i0;
+    load4<T, VEC>(x, x0);
+    load4<T, VEC>(x + HALF, x1);
+  }
+  if (rotated) {
+    const float* w = (h < a.H ? a.q_norm : a.k_norm) + i0;
+    load4<float, VEC>(w, w0);
+    load4<float, VEC>(w + HALF, w1);
+  }
   int64_t at = -1;
   bool bad = pos >= a.n_pos;
   if (a.kc) {
@@ -87,72 +102,50 @@ __global__ void __launch_bounds__(kNrThreads)
     if (at >= a.n_rows) at = -1;
   }
   if (bad && threadIdx.x == 0 && blockIdx.y == 0 && a.status) atomicCAS(a.status, 0, kStatusBadIndex);
-  if (!in_table) return;  // padding (pos < 0) or refused: nothing of this token is written
-  const T* row = static_cast<const T*>(a.qkv) + static_cast<int64_t>(t) * a.ld;
-  const int i0 = 4 * lane;
-  float c[4], s[4];
-  {
-    const float* cs = a.rope + static_cast<int64_t>(pos) * D;
+  if (pos < 0 || pos >= a.n_pos) return;  // padding or refused: nothing of this token is written
+  float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = cs[i0 + i], s[i] = cs[HALF + i0 + i];
-  }
-  // every lane of a warp runs every round, so the shuffles see whole warps
-  for (int h0 = blockIdx.y * GROUPS; h0 < heads; h0 += gridDim.y * GROUPS) {
-    const int h = h0 + group;
-    const bool on = h < heads;
-    float x0[4] = {}, x1[4] = {};
-    if (on) {
-      const T* x = row + static_cast<int64_t>(h) * D;
-      load4<T, VEC>(x + i0, x0);
-      load4<T, VEC>(x + HALF + i0, x1);
+  for (int i = 0; i < 4; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+  ss = group_sum<LANES>(ss);
+  if (rotated) {
+    const float* cs = a.rope + static_cast<int64_t>(pos) * D + i0;
+    float c[4], s[4];
+    load4<float, VEC>(cs, c);
+    load4<float, VEC>(cs + HALF, s);
+    const float r = rsqrtf(ss * (1.0f / D) + a.eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y0 = x0[i] * r * w0[i], y1 = x1[i] * r * w1[i];
+      x0[i] = y0 * c[i] - y1 * s[i];
+      x1[i] = y0 * s[i] + y1 * c[i];
     }
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
-    ss = group_sum<LANES>(ss);
-    if (h < a.H + a.KV) {
-      const float* w = h < a.H ? a.q_norm : a.k_norm;
-      const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y0 = x0[i] * r * w[i0 + i], y1 = x1[i] * r * w[HALF + i0 + i];
-        x0[i] = y0 * c[i] - y1 * s[i];
-        x1[i] = y0 * s[i] + y1 * c[i];
-      }
-    }
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(x0[i]), fabsf(x1[i])));
-    amax = group_max<LANES>(amax);
-    if (!on) continue;
-    if (h < a.H + a.KV) {
-      T* out = h < a.H ? static_cast<T*>(a.q) + static_cast<int64_t>(t) * a.q_ld + static_cast<int64_t>(h) * D
-                       : static_cast<T*>(a.k) + static_cast<int64_t>(t) * a.k_ld + static_cast<int64_t>(h - a.H) * D;
-      if (h < a.H || a.k) {
-        store4<T, VEC>(out + i0, x0);
-        store4<T, VEC>(out + HALF + i0, x1);
-      }
-    }
-    if (a.kc && h >= a.H && at >= 0) {
-      const bool is_k = h < a.H + a.KV;
-      const int kvh = is_k ? h - a.H : h - a.H - a.KV;
-      const int64_t r = static_cast<int64_t>(kvh) * a.n_rows + at;
-      const float d = __fdiv_rn(amax, 127.0f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-      int8_t* q8 = (is_k ? a.kc : a.vc) + r * D;
-      store_i8x4(q8 + i0, x0, id);
-      store_i8x4(q8 + HALF + i0, x1, id);
-      if (lane == 0) (is_k ? a.ks : a.vs)[r] = d;
+    T* out = h < a.H ? static_cast<T*>(a.q) + static_cast<int64_t>(t) * a.q_ld + static_cast<int64_t>(h) * D
+                     : static_cast<T*>(a.k) + static_cast<int64_t>(t) * a.k_ld + static_cast<int64_t>(h - a.H) * D;
+    if (h < a.H || a.k) {
+      store4<T, VEC>(out + i0, x0);
+      store4<T, VEC>(out + HALF + i0, x1);
     }
   }
+  if (at < 0) return;  // the whole block: no cache row for this token
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(x0[i]), fabsf(x1[i])));
+  amax = group_max<LANES>(amax);
+  if (!on || h < a.H) return;
+  const int kvh = rotated ? h - a.H : h - a.H - a.KV;
+  const int64_t r = static_cast<int64_t>(kvh) * a.n_rows + at;
+  const float d = __fdiv_rn(amax, 127.0f), id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+  int8_t* q8 = (rotated ? a.kc : a.vc) + r * D;
+  store_i8x4(q8 + i0, x0, id);
+  store_i8x4(q8 + HALF + i0, x1, id);
+  if (lane == 0) (rotated ? a.ks : a.vs)[r] = d;
 }
 
 template <typename T, int D>
-void run_norm_rope(const NormRopeArgs& a, bool vec, int sms, cudaStream_t s) {
+void run_norm_rope(const NormRopeArgs& a, bool vec, cudaStream_t s) {
   constexpr int GROUPS = kNrThreads / (D / 8);
   const int heads = a.H + a.KV + (a.kc ? a.KV : 0);
-  const int slices = (heads + GROUPS - 1) / GROUPS;
-  const dim3 grid(static_cast<unsigned>(a.n), static_cast<unsigned>(slices));
-  (void)sms;
+  const dim3 grid(static_cast<unsigned>(a.n), static_cast<unsigned>((heads + GROUPS - 1) / GROUPS));
   if (vec)
     k_qk_norm_rope<T, D, true><<<grid, kNrThreads, 0, s>>>(a);
   else
@@ -160,25 +153,26 @@ void run_norm_rope(const NormRopeArgs& a, bool vec, int sms, cudaStream_t s) {
 }
 
 template <typename T>
-void run_norm_rope_d(const NormRopeArgs& a, int D, bool vec, int sms, cudaStream_t s) {
-  if (D == 64) return run_norm_rope<T, 64>(a, vec, sms, s);
-  if (D == 128) return run_norm_rope<T, 128>(a, vec, sms, s);
-  run_norm_rope<T, 256>(a, vec, sms, s);
+void run_norm_rope_d(const NormRopeArgs& a, int D, bool vec, cudaStream_t s) {
+  if (D == 64) return run_norm_rope<T, 64>(a, vec, s);
+  if (D == 128) return run_norm_rope<T, 128>(a, vec, s);
+  run_norm_rope<T, 256>(a, vec, s);
 }
 
 }  // namespace
 
-void launch_qk_norm_rope(const NormRopeArgs& a, ActType type, int D, int sms, cudaStream_t s) {
+void launch_qk_norm_rope(const NormRopeArgs& a, ActType type, int D, cudaStream_t s) {
   if (a.n <= 0) return;
-  // whole words when every row of every buffer starts on one (rows are D apart inside a token, ld apart between them)
-  const int word = type == ActType::f32 ? 16 : 8;
-  auto whole = [&](const void* p, int64_t ld) {
+  // whole words when every row of every buffer starts on one (heads are D apart inside a token, tokens ld)
+  auto whole = [](const void* p, int64_t ld, int word) {
     return !p || (reinterpret_cast<uintptr_t>(p) % word == 0 && ld % 4 == 0);
   };
-  const bool vec = whole(a.qkv, a.ld) && whole(a.q, a.q_ld) && whole(a.k, a.k_ld);
-  if (type == ActType::f32) return run_norm_rope_d<float>(a, D, vec, sms, s);
-  if (type == ActType::f16) return run_norm_rope_d<__half>(a, D, vec, sms, s);
-  run_norm_rope_d<__nv_bfloat16>(a, D, vec, sms, s);
+  const int word = type == ActType::f32 ? 16 : 8;
+  const bool vec = whole(a.qkv, a.ld, word) && whole(a.q, a.q_ld, word) && whole(a.k, a.k_ld, word) &&
+                   whole(a.rope, 0, 16) && whole(a.q_norm, 0, 16) && whole(a.k_norm, 0, 16);
+  if (type == ActType::f32) return run_norm_rope_d<float>(a, D, vec, s);
+  if (type == ActType::f16) return run_norm_rope_d<__half>(a, D, vec, s);
+  run_norm_rope_d<__nv_bfloat16>(a, D, vec, s);
 }
 
 }  // namespace mkb
