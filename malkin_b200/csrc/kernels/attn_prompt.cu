@@ -65,7 +65,7 @@ constexpr int prompt_smem() {
 }
 
 // The sequence and the 256-row tile that CTA `want` of a head takes: of each 32 sequences the tiles with the most keys first,
-// so that what runs last is short (in sequence order the eight packed prompts of the table took YY us for XX). A tile's place
+// so that what runs last is short (eight prompts of up to 2048 tokens, 32 heads of 128: 225 us for 229 in sequence order). A tile's place
 // is found from the number of tiles at or above a depth, by bisection.
 __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, int want, int lane, int* status,
                                           PromptSmall* sm) {
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         s[i] = f2_lo(x);
         s[i + 1] = f2_hi(x);
       }
-      constexpr int kLag = 8;  // exponentials in flight
+      constexpr int kLag = 8;  // exponentials ahead of their sums and packing
       uint32_t p[16];
 #pragma unroll
       for (int i = 0; i < kKeys + kLag; i += 2) {

@@ -86,28 +86,6 @@ __device__ __forceinline__ bool mbar_wait_warp_sleep(uint64_t* bar, uint32_t par
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
-// Waits for kernels whose warps wait most of the time: each try suspends the warp for up to kParkNs (or until the phase
-// completes) instead of coming back at once, so that the waiting warps leave the issue slots to the working ones (polls were
-// half of the attention kernels' instructions). At most kParkLimit tries, about a second.
-constexpr uint32_t kParkNs = 20000, kParkLimit = 1u << 16;
-__device__ __forceinline__ bool mbar_park(uint64_t* bar, uint32_t parity, int* status, int code) {
-  for (uint32_t i = 0; i < kParkLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(kParkNs)
-        : "memory");
-    if (ok) return true;
-  }
-  if (status) atomicCAS(status, 0, code);
-  return false;
-}
-// By a whole warp, with one outcome for every lane.
-__device__ __forceinline__ bool mbar_park_warp(uint64_t* bar, uint32_t parity, int* status, int code) {
-  return __all_sync(0xffffffffu, mbar_park(bar, parity, status, code)) != 0;
-}
-
 // 1-D bulk copy global -> shared, completion counted in bytes on bar. dst, src 16-byte aligned; bytes % 16 == 0.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(

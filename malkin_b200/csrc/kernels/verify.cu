@@ -16,7 +16,7 @@
 // A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the
 // row's exponentials and sums are in 64 bits: with 32 the drawn index would differ from the exact one about once in 10^4
 // draws. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
-// slower: 93, 85 and 96 us against 72 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
+// slower: 93, 85 and 96 us against 75 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

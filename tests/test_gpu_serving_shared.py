@@ -6,10 +6,10 @@ pytestmark = pytest.mark.gpu
 
 F16, BF16 = 1, 30
 
-# Error of an output beside A = sum_j w_j |v_j|: weights x scales are rounded to bf16 (2^-8 of each); fp32 parts (scores of
+# Error of an output beside A = sum_j w_j |v_j|: weights x scales are rounded to fp16 (2^-11 of each); fp32 parts (scores of
 # D products, exponents, sums, joining) together below 2^-11 A for scores below 24, as in the prompt attention's test;
 # then half a step of the output's type.
-W_PART = 2.0 ** -8 + 2.0 ** -11
+W_PART = 2.0 ** -11 + 2.0 ** -11
 
 
 def tt(torch, t):
@@ -170,6 +170,22 @@ def test_rising_maximum(mk, torch_cuda):
     b.k[0, lo + 1999] = 127
     q = (queries(torch, BF16, b.n, H, D, 2).float().abs() * 0.1).to(torch.bfloat16)
     check(torch, BF16, b, q, call(mk, torch, BF16, b, q, H, KV, D), H, KV, D)
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("H,KV,D", [(8, 2, 128), (16, 8, 64), (5, 1, 128)])
+def test_pieces_of_every_length(mk, torch_cuda, t, H, KV, D):
+    """Batches whose parts are one block or many, alone and dual, so that pieces end at every place in a unit."""
+    torch = torch_cuda
+    for seed in range(4):
+        rng = np.random.default_rng(seed)
+        groups = []
+        for _ in range(int(rng.integers(1, 6))):
+            reqs = [(int(rng.integers(0, 400)), int(rng.integers(1, 5))) for _ in range(int(rng.integers(1, 24)))]
+            groups.append((int(rng.integers(0, 1500)) if rng.random() < 0.7 else int(rng.integers(0, 97)), reqs))
+        b = Batch(rng, groups, KV, D, loose=seed)
+        q = queries(torch, t, b.n, H, D, seed)
+        check(torch, t, b, q, call(mk, torch, t, b, q, H, KV, D), H, KV, D)
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
