@@ -601,8 +601,7 @@ int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int
                {dev_status, 4, "dev_status", true}}, who);
     mkb::NormRopeArgs a{dev_qkv, ld, n, H, KV, dev_q_norm, dev_k_norm, eps, dev_rope, n_pos, dev_pos, dev_q, q_ld,
                         dev_k, k_ld, dev_kc, dev_vc, dev_ks, dev_vs, n_rows, dev_kv_at, dev_status};
-    mkb::launch_qk_norm_rope(a, t, D, as_stream(stream));
-    mkb::cuda_check(cudaGetLastError(), who);
+    mkb::cuda_check(static_cast<cudaError_t>(mkb::launch_qk_norm_rope(a, t, D, current_sms(), as_stream(stream))), who);
   });
 }
 

@@ -267,7 +267,7 @@ struct NormRopeArgs {
   const int32_t* kv_at;
   int* status;
 };
-void launch_qk_norm_rope(const NormRopeArgs& a, ActType type, int D, cudaStream_t s);
+int launch_qk_norm_rope(const NormRopeArgs& a, ActType type, int D, int sms, cudaStream_t s);
 
 struct VerifyArgs {
   const void* logits;  // [n_rows][ld]

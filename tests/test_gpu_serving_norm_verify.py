@@ -137,6 +137,59 @@ def test_norm_rope_in_place_with_cache(mk, torch_cuda, t, D):
                 assert (q8[:, r] == 99).all() and (sc[:, r] == -1).all()
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("H,KV,D,cache,inplace", [(32, 8, 128, True, False), (32, 8, 128, False, True), (24, 8, 64, True, True),
+                                                  (7, 3, 256, True, False), (64, 8, 64, False, False), (5, 1, 64, True, False)])
+def test_norm_rope_large_batches(mk, torch_cuda, t, H, KV, D, cache, inplace):
+    """A large batch gives the bits that its tokens give in small ones, padding, refused indexes and untouched rows among them;
+    the first and last tokens against the 64-bit form."""
+    torch = torch_cuda
+    n, rows, n_pos = 4001, 5000, 500
+    ld = (H + 2 * KV) * D + 16
+    _, x = norm_inputs(torch, t, n, H, KV, D, ld, 0, 3)
+    before = x.clone()
+    g = torch.Generator().manual_seed(8)
+    qw, kw = ((1 + 0.3 * torch.randn(D, generator=g)).cuda() for _ in range(2))
+    ang = torch.rand(n_pos, D // 2, generator=g) * 6
+    rope = torch.cat([ang.cos(), ang.sin()], 1).contiguous().cuda()
+    pos = torch.randint(0, n_pos, (n,), generator=g).int()
+    pos[[5, 700, 3999]] = torch.tensor([-1, n_pos, -7]).int()
+    at = torch.randperm(rows, generator=g)[:n].int()
+    at[[6, 1700]] = torch.tensor([-1, rows]).int()
+    pos, at = pos.cuda(), at.cuda()
+
+    def call(step):
+        src = before.clone()
+        q, k = (torch.full((n, w * D), 7.0, dtype=x.dtype, device="cuda") for w in (H, KV))
+        qp, kp, q_ld, k_ld = q.data_ptr(), k.data_ptr(), H * D, KV * D
+        e = src.element_size()
+        if inplace:
+            qp, kp, q_ld, k_ld = src.data_ptr(), src.data_ptr() + H * D * e, ld, ld
+        kc, vc = (torch.full((KV, rows, D), 99, dtype=torch.int8, device="cuda") for _ in range(2))
+        ks, vs = (torch.full((KV, rows), -1.0, device="cuda") for _ in range(2))
+        st = torch.zeros(1, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        for lo in range(0, n, step):
+            held = (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), rows, at.data_ptr() + 4 * lo) if cache else ()
+            mk.qk_norm_rope(t, src.data_ptr() + lo * ld * e, ld, min(step, n - lo), H, KV, D, qw.data_ptr(), kw.data_ptr(),
+                            1e-6, rope.data_ptr(), n_pos, pos.data_ptr() + 4 * lo, qp + lo * q_ld * e, q_ld,
+                            kp + lo * k_ld * e, k_ld, *held, dev_status=st.data_ptr())
+        torch.cuda.synchronize()
+        assert int(st) == mk.MK_ERR_ARG
+        if inplace:
+            q, k = src[:, :H * D], src[:, H * D:(H + KV) * D]
+        return [a.contiguous().view(torch.uint8) for a in (src, q, k, kc, vc, ks, vs)] + [host(q), host(k)]
+
+    large, small = call(n), call(97)
+    for a, b in zip(large[:7], small[:7]):
+        assert torch.equal(a, b)
+    for i in (0, n - 1):
+        heads = host(before[i, :(H + KV) * D]).reshape(-1, D)
+        for got, lo, m, w in ((large[7], 0, H, qw), (large[8], H, KV, kw)):
+            y, terms = ref.norm_rope(heads[lo:lo + m], host(w), 1e-6, host(rope[int(pos[i])]))
+            check_norm(torch, t, got[i].reshape(-1, D), y, terms)
+
+
 # ---------------- verification ----------------
 # p of a draft: its own exponential is in 64 bits, the row's sum is of 32-bit exponentials 2^t: t carries two roundings
 # (2^-23 |t| ln 2 relative), entries below 2^-40 of the maximum weigh nothing, exp2f is good to 2 steps, sums and the
