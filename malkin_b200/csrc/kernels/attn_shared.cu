@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstddef>
 #include <type_traits>
 
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
         x.own = 0;
       }
     }
-    n_tiles += total;
+    n_tiles = min(n_tiles + total, w.prefix_tiles + 1);  // a round adds at most 2^29
   }
   if (n_tiles > w.prefix_tiles) {  // groups that overlap one another: no result
     for (int t = tid; t < a.n; t += kPlanThreads) w.tok_own[t] = -1;
@@ -281,7 +282,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
   }
   const int open = places < static_cast<int64_t>(kFewBlocks) * ctas ? 0 : kOpen;
   places += open * n_units;
-  const int per = static_cast<int>(max(static_cast<int64_t>(open + 1), (places + ctas - 1) / ctas));
+  const int64_t longest = max(static_cast<int64_t>(open + 1), (places + ctas - 1) / ctas);
+  const bool too_long = longest > INT_MAX;  // hours of work; a piece's places are counted in 32 bits
+  const int per = too_long ? 1 : static_cast<int>(longest);
+  bad |= too_long;
   int64_t rows = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
     if (i < n_tiles) w.tile[i].row = rows + incl - mine;
     rows += total;
   }
-  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows ? places : 0, open};
+  if (tid == 0) *w.head = PlanHead{n_tiles, per, rows <= w.rows && !too_long ? places : 0, open};
   if (bad && a.status) atomicCAS(a.status, 0, kStatusBadIndex);
 }
 

@@ -178,3 +178,65 @@ def test_step_captured_beside_another(mk, torch_cuda):
             torch.cuda.synchronize()
             for a, b in zip(first, s.results()):
                 assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(mk, torch_cuda):
+    """Buffers of more than 2^32 bytes and 2^31 elements, used at their far ends."""
+    torch = torch_cuda
+    d = lambda a, dt=torch.int32: torch.as_tensor(np.asarray(a)).to(dt).cuda()  # noqa: E731
+    st, g = d([0]), torch.Generator().manual_seed(1)
+    # rows 2^22 elements apart, 600 of them: prompt attention and the norm in place, then its cache rows far out
+    ld, n, rows = 1 << 22, 600, 18_000_000
+    x = torch.empty(n * ld, dtype=torch.bfloat16, device="cuda").view(n, ld)
+    x[:, :WIDE] = torch.randn(n, WIDE, generator=g).bfloat16().cuda()
+    kc, vc = (torch.empty(KV, rows, D, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(KV, rows, dtype=torch.float32, device="cuda") for _ in range(2))
+    assert x.numel() > 2 ** 31 and kc.numel() > 2 ** 32
+    raw = x[:, :WIDE].float().cpu().numpy()
+    ang = torch.rand(n, D // 2, generator=g) * 6
+    rope = torch.cat([ang.cos(), ang.sin()], 1).contiguous().cuda()
+    w, pos, at = torch.ones(D, device="cuda"), d(np.arange(n)), d(np.arange(rows - n, rows))
+    e = 2
+    mk.qk_norm_rope(BF16, x.data_ptr(), ld, n, H, KV, D, w.data_ptr(), w.data_ptr(), 1e-6, rope.data_ptr(), n,
+                    pos.data_ptr(), x.data_ptr(), ld, x.data_ptr() + H * D * e, ld, kc.data_ptr(), vc.data_ptr(),
+                    ks.data_ptr(), vs.data_ptr(), rows, at.data_ptr(), st.data_ptr())
+    torch.cuda.synchronize()
+    got = x[:, :WIDE].float().cpu().numpy()
+    for i in (0, n - 1):
+        y, terms = ref.norm_rope(raw[i].reshape(-1, D)[:H + KV], np.ones(D), 1e-6, rope[i].cpu().numpy())
+        check_norm(torch, BF16, got[i].reshape(-1, D)[:H + KV], y, terms)
+        held = vc[:, rows - n + i].cpu().numpy() * vs[:, rows - n + i].cpu().numpy()[:, None]
+        v = raw[i].reshape(-1, D)[H + KV:]
+        assert np.all(np.abs(held - v) <= np.abs(v).max(-1, keepdims=True) / 127 * 0.5001)
+    out = x[:, WIDE:WIDE + H * D]
+    off = d([0, 300, 600])
+    mk.attention_prompt(BF16, x.data_ptr(), ld, x.data_ptr() + H * D * e, ld, x.data_ptr() + (H + KV) * D * e, ld, n, 2,
+                        off.data_ptr(), H, KV, D, D ** -0.5, out.data_ptr(), ld, st.data_ptr())
+    torch.cuda.synchronize()
+    check_prompt(torch, BF16, got.astype(np.float64), off.cpu().numpy(), out.float().cpu().numpy(), H, KV, D)
+    # the far rows as a prefix of 500 and own rows behind it
+    tok = 4
+    b = types.SimpleNamespace(n=tok, k=kc[:, rows - n:].cpu().numpy(), v=vc[:, rows - n:].cpu().numpy(),
+                              ks=ks[:, rows - n:].cpu().numpy(), vs=vs[:, rows - n:].cpu().numpy())
+    b.keys_of = lambda i: list(range(500 + i)) + [n - 1]
+    args = [d(a) for a in ([0, tok], [rows - n], [500], [rows - n + 500] * tok, range(tok), range(tok + 1), [99] * tok)]
+    y = torch.empty(tok, H * D, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(mk.attention_shared_workspace(tok, H, KV, D, 1), dtype=torch.uint8, device="cuda")
+    mk.attention_shared(BF16, x.data_ptr() + (n - tok) * ld * e, ld, tok, H, KV, D, D ** -0.5, kc.data_ptr(),
+                        vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), rows, 1, *[a.data_ptr() for a in args], tok,
+                        y.data_ptr(), H * D, ws.data_ptr(), ws.numel(), st.data_ptr())
+    torch.cuda.synchronize()
+    check_shared(torch, BF16, b, x[n - tok:, :H * D], y.float().cpu().numpy(), H, KV, D)
+    # logits rows that far apart
+    lg = x[:, :V]
+    lg[n - 3:] = (torch.randn(3, V, generator=g) * 3).bfloat16().cuda()
+    row_off, draft = d([0, 597, 600]), d(np.arange(598) % V)
+    u, temp = torch.rand(n, generator=g, dtype=torch.float64).cuda(), torch.ones(2, device="cuda")
+    n_acc, nxt, p = d([0, 0]), d([0, 0]), torch.empty(598, device="cuda")
+    wv = torch.empty(mk.verify_draft_workspace(n, 2, V), dtype=torch.uint8, device="cuda")
+    mk.verify_draft(BF16, x.data_ptr(), ld, n, V, 2, row_off.data_ptr(), draft.data_ptr(), 0, 0, temp.data_ptr(),
+                    u.data_ptr(), n_acc.data_ptr(), nxt.data_ptr(), p.data_ptr(), wv.data_ptr(), wv.numel(), st.data_ptr())
+    torch.cuda.synchronize()
+    want = ref.verify(lg.float().cpu().numpy().astype(np.float64), [0, 597, 600], draft.cpu().numpy(), None,
+                      [1.0, 1.0], u.cpu().numpy())
+    check_verify((n_acc.cpu().numpy(), nxt.cpu().numpy(), p.cpu().numpy(), int(st)), want, 598)

@@ -258,6 +258,9 @@ def test_bad_tables(mk, torch_cuda):
     b.group_off = [0, 7, 0, 7, 0, 7]
     b.prefix_base, b.prefix_len = [5] * 5, [30] * 5
     call(mk, torch, BF16, b, q, H, KV, D, status=mk.MK_ERR_ARG)
+    b.group_off = [0, 7] * 1300
+    b.prefix_base, b.prefix_len = [5] * 2599, [30] * 2599
+    call(mk, torch, BF16, b, q, H, KV, D, status=mk.MK_ERR_ARG)
 
 
 def test_streams_and_graph(mk, torch_cuda):
