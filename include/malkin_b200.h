@@ -354,7 +354,8 @@ int mk_attention(const float* dev_q, int n, int H, int KV, int D, const int8_t* 
  * key head and the value head of token t are quantized (quantize_i8, quant.cpp:134-140) from their fp32 values into row
  * dev_kv_at[t]. Two tokens with the same row leave either's values there.
  * A token with dev_pos[t] < 0 is padding: nothing of it is written; dev_kv_at[t] < 0: no cache row of it is written.
- * dev_pos[t] >= n_pos or dev_kv_at[t] >= n_rows does the same and records MK_ERR_ARG. */
+ * dev_pos[t] >= n_pos or dev_kv_at[t] >= n_rows does the same and records MK_ERR_ARG. A token's results do not depend on
+ * the batch it is in. MK_ERR_TIMEOUT (recorded): a wait inside the kernel ran out, the outputs are not valid. */
 int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int KV, int D, const float* dev_q_norm,
                     const float* dev_k_norm, float eps, const float* dev_rope, int n_pos, const int32_t* dev_pos,
                     void* dev_q, int64_t q_ld, void* dev_k, int64_t k_ld, int8_t* dev_kc, int8_t* dev_vc, float* dev_ks,

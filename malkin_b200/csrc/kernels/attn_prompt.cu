@@ -65,8 +65,8 @@ constexpr int prompt_smem() {
 }
 
 // The sequence and the 256-row tile that CTA `want` of a head takes: of each 32 sequences the tiles with the most keys first,
-// so that what runs last is short (eight prompts of up to 2048 tokens, 32 heads of 128: 225 us for 229 in sequence order). A tile's place
-// is found from the number of tiles at or above a depth, by bisection.
+// so that what runs last is short (eight prompts of up to 2048 tokens, 32 heads of 128: 225 us for 229 in sequence order). A
+// tile's place is found from the number of tiles at or above a depth, by bisection.
 __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, int want, int lane, int* status,
                                           PromptSmall* sm) {
   int lo_f = 0, hi_f = 0, tile_f = -1;

@@ -91,8 +91,8 @@ __device__ __forceinline__ void store_i8(int8_t* p, const float (&v)[kVals], flo
 // warps call it, with on false in lanes without a head; `cache` is the same for all of a warp.
 template <typename T, int D, bool VEC>
 __device__ __forceinline__ void finish_head(const NormRopeArgs& a, int t, int h, int lane, bool on, bool cache, int64_t at,
-                                            float (&x0)[kVals], float (&x1)[kVals], const float (&w0)[kVals], const float (&w1)[kVals],
-                                            const float (&c)[kVals], const float (&s)[kVals]) {
+                                            float (&x0)[kVals], float (&x1)[kVals], const float (&w0)[kVals],
+                                            const float (&w1)[kVals], const float (&c)[kVals], const float (&s)[kVals]) {
   constexpr int LANES = D / (2 * kVals), HALF = D / 2;
   const int i0 = kVals * lane;
   const bool rotated = h < a.H + a.KV;
@@ -278,7 +278,8 @@ __global__ void __launch_bounds__(kRingThreads, kRingCtas) k_qk_norm_rope_ring(N
           load<float, true>(w, w0);
           load<float, true>(w + HALF, w1);
         }
-        finish_head<T, D, true>(a, static_cast<int>(t), h, lane, on, at >= 0 && h0 + (warp + 1) * (32 / LANES) > a.H, at, x0, x1, w0, w1, c, s);
+        const bool cache = at >= 0 && h0 + (warp + 1) * (32 / LANES) > a.H;  // the warp has key or value heads
+        finish_head<T, D, true>(a, static_cast<int>(t), h, lane, on, cache, at, x0, x1, w0, w1, c, s);
       }
     }
     __syncwarp();

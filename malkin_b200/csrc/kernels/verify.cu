@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_verify_rows(VerifyArgs a, in
     before += __syncthreads_count(r0 + tid < a.n_req && a.row_off[r0 + tid + 1] <= row);
   const float T0 = before < a.n_req ? a.temperature[before] : 0.0f;
   const bool sums = T0 > 0.0f;  // rows of a greedy request need the index of the maximum, the others the sum
-  const float c = sums ? fminf(1.44269504088896341f / T0, FLT_MAX) : 0.0f;  // exp(x / T) = 2^(x c)
+  // exp(x / T) = 2^(x c); above 0, so that -infinity keeps its weight 0 where T is infinite
+  const float c = sums ? fmaxf(fminf(1.44269504088896341f / T0, FLT_MAX), FLT_MIN) : 0.0f;
   float mx = -INFINITY, sum = 0.0f;
   int idx = INT32_MAX;
   for (int64_t at = begin; at < end; at += kRowTile) {

@@ -325,6 +325,26 @@ def test_verify_edges(mk, torch_cuda):
     assert got[1][0] >= 290 and got[1][14] >= 290 and got[1][14] != 295
 
 
+@pytest.mark.parametrize("temp", [float("inf"), 3e38, 1e-38])
+def test_verify_extreme_temperatures(mk, torch_cuda, temp):
+    """Towards infinity every token that can be drawn weighs the same, towards 0 the maximum takes all."""
+    torch = torch_cuda
+    V = 5003
+    logits = torch.randn(3, V, generator=torch.Generator().manual_seed(1)).cuda()
+    logits[:, 1::2] = -float("inf")
+    top = int(logits[0].argmax())
+    some = (V + 1) // 2
+    got = verify_call(mk, torch, F32, logits, V, [0, 2, 3], [top], None, 0, [temp, temp], [0.0, 0.5, 0.25], V, 2)
+    assert got[3] == 0 and list(got[0]) == [1, 0]
+    want = [int(logits[1].argmax()), int(logits[2].argmax())]
+    if temp > 1:
+        assert abs(got[2][0] - 1 / some) <= P_REL / some
+        want = [2 * (-(-some // 2) - 1), 2 * (-(-some // 4) - 1)]  # the first whose rank reaches u x some
+    else:
+        assert got[2][0] == 1
+    assert list(got[1]) == want
+
+
 def test_verify_bad_tables(mk, torch_cuda):
     """Offsets that run backwards, past the rows or below zero: those requests give (0, -1) and the status, the others
     their results."""
