@@ -13,8 +13,8 @@
 //                        blocks whose bytes are in flight only a part of their life, so large batches stop at half of HBM:
 //                        16384 tokens of 32 + 8 + 8 heads of 128, bf16 with cache rows: 115 us (3.5 TB/s)
 //   k_qk_norm_rope_ring  large batches of wide rows: whole rows by bulk copies ahead of eight warps: 90 us (4.5 TB/s); with
-//                        40 + 8 + 8 heads of 256 160 us (5.9 TB/s) against 270. What holds it is the latency of a head's
-//                        chain (two butterflies, a root, two divisions) in the 24 warps that fit beside the rows
+//                        40 + 8 + 8 heads of 256 160 us (5.9 TB/s) against 270. What holds it is issue (70 % of the slots)
+//                        and the latency of a head's chain in the 24 warps that fit beside the rows
 // The rule: rows of at least 4 KB (rows of 3 KB: 41 us against 32, of 6 KB: 60 against 70, 16384 tokens) and at least eight
 // of them for each CTA (2048 tokens of 12 KB: 15.5 us against 14.2, 4096: 26.4 against 28.5).
 // Not kept: eight values a lane (16-byte words of 16-bit types; 109 us for 104 without the ring, 103 for 90 with it), two,
