@@ -352,7 +352,7 @@ int mk_attention(const float* dev_q, int n, int H, int KV, int D, const int8_t* 
  * In place is allowed: dev_q = dev_qkv with q_ld = ld, dev_k = its key heads with k_ld = ld.
  * dev_kc / dev_vc (NULL: no cache): int8 [KV][n_rows][D] with float row scales dev_ks / dev_vs [KV][n_rows]; the rotated
  * key head and the value head of token t are quantized (quantize_i8, quant.cpp:134-140) from their fp32 values into row
- * dev_kv_at[t]. Two tokens with the same row leave either's values there.
+ * dev_kv_at[t]. A row that two tokens name holds a mixture of both.
  * A token with dev_pos[t] < 0 is padding: nothing of it is written; dev_kv_at[t] < 0: no cache row of it is written.
  * dev_pos[t] >= n_pos or dev_kv_at[t] >= n_rows does the same and records MK_ERR_ARG. A token's results do not depend on
  * the batch it is in. MK_ERR_TIMEOUT (recorded): a wait inside the kernel ran out, the outputs are not valid. */

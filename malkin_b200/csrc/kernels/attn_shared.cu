@@ -18,7 +18,11 @@
 // but that plus the exponent of the block's largest V scale, less 6: products are at most 2^15, and full precision reaches
 // down to 2^-20 of the largest. Sums and outputs carry the same reference, so it cancels.
 // Bound: HBM for one tile of rows a group (128 rows: 65.5 kFLOP against 264 bytes a key and head, the machine's balance),
-// the tensor pipe and the conversion above that.
+// the tensor pipe and the conversion above that. What holds it: a block of 96 keys takes 3700 cycles for 128 rows and 3900 for
+// 256, 2500 of them the widening (K to bf16 1700, V to fp16 800); the plan takes 7 us, finding a piece's place 2, the join 4 to
+// 5. Measured, with queries of 32 / 8 heads of 128: two prefixes of up to 32768 rows with 32 requests of 4 rows each, bf16:
+// 246 to 252 us; 8 trees of 17 rows behind 2048 rows, fp16: 44; 4 single rows behind 1000, 16 / 8 heads, bf16: 25. Two CTAs an
+// SM with blocks of 64 keys took 497 us at the first.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
