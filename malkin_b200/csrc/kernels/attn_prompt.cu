@@ -19,8 +19,8 @@
 // blocks of 128 keys 3670 cycles, of which the softmax takes 2200 and the four MMAs 1320, little of it at once, because both
 // tiles' S and O fill TMEM and no scores can be computed ahead. Measured: 8192 tokens, 40 / 8 heads of 128, fp16: 614 to
 // 622 us (1.1 PFLOP/s) in bursts, 710 in a loop of seconds, under the power limit; eight prompts of up to 2048 tokens, 32 / 8
-// heads, bf16: 209 to 220 us. Not kept, at the long prompt: two threads a row 692 us; 64-key blocks with S in two buffers 777; 2^x by a polynomial
-// on the FMA pipe for 1/4 of the weights 626 against 632 in the same run, for 3/8 664.
+// heads, bf16: 209 to 220 us. Not kept, at the long prompt: two threads a row 692 us; 64-key blocks with S in two buffers 777;
+// 2^x by a polynomial on the FMA pipe for 1/4 of the weights 626 against 632 in the same run, for 3/8 664.
 //
 // Masked keys: scores above the diagonal are replaced by -inf, whatever K holds there. Their weight 0 would still make a
 // NaN of an infinity or NaN in V, so the tiles on the diagonal, whose keys some rows must not see (later tokens, or the
