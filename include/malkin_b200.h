@@ -415,7 +415,8 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
  * looked at, 0 for those after the first one that was not kept. A draft outside 0 .. V - 1 has probability 0. Logits of
  * -infinity are tokens that cannot be drawn, NaN logits count as -infinity; a row whose maximum is not finite has no
  * distribution: no draft is kept on it, and as the row drawn from it gives dev_next = -1. A request whose rows are not as
- * above gives dev_n_acc = 0, dev_next = -1 and records MK_ERR_ARG (its dev_p entries are not written).
+ * above, or that has rows or drafts of an earlier one whose rows are in the buffers, gives dev_n_acc = 0, dev_next = -1 and
+ * records MK_ERR_ARG (its dev_p entries are not written); the others are not changed by it.
  * dev_ws: mk_verify_draft_workspace(n_rows, n_req, V) bytes, 16-byte aligned. V at most 2^27, n_req at most 65535. */
 int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V);
 int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,

@@ -66,6 +66,11 @@ int verify_chunk_tiles(int n_rows, int V, int sms) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(per, kRowTilesMax)));
 }
 
+// The rows of request r lie in the buffers, and so do its drafts (row x of it has draft x - r).
+__device__ __forceinline__ bool rows_fit(const VerifyArgs& a, int r, int lo, int hi) {
+  return lo >= r && hi > lo && hi <= a.n_rows && hi - 1 - r <= a.n_rows - a.n_req;
+}
+
 __device__ __forceinline__ bool above(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
 
 template <typename T>
@@ -88,6 +93,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_verify_rows(VerifyArgs a, in
   __shared__ float s_mx[kRowThreads / 32];
   __shared__ int s_idx[kRowThreads / 32];
   __shared__ double s_sum[kRowThreads / 32];
+  __shared__ int s_req;
   const int row = blockIdx.x, chunk = blockIdx.y, tid = threadIdx.x;
   const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(row) * a.ld;
   const int64_t begin = static_cast<int64_t>(chunk) * tiles * kRowTile;
@@ -111,11 +117,16 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_verify_rows(VerifyArgs a, in
     }
   };
   load(begin);
-  // the row's request: offsets ascend, so it is the number of requests that end at or before the row
-  int before = 0;
-  for (int r0 = 0; r0 < a.n_req; r0 += kRowThreads)
-    before += __syncthreads_count(r0 + tid < a.n_req && a.row_off[r0 + tid + 1] <= row);
-  const float T0 = before < a.n_req ? a.temperature[before] : 0.0f;
+  // the row's request: the first one whose own offsets hold it. A request that is not refused has no row of an earlier one
+  // that fits, so offsets that are wrong elsewhere do not change it.
+  if (tid == 0) s_req = a.n_req;
+  __syncthreads();
+  for (int r = tid; r < a.n_req; r += kRowThreads) {
+    const int lo = a.row_off[r], hi = a.row_off[r + 1];
+    if (row >= lo && row < hi && rows_fit(a, r, lo, hi)) atomicMin(&s_req, r);
+  }
+  __syncthreads();
+  const float T0 = s_req < a.n_req ? a.temperature[s_req] : 0.0f;
   const bool sums = T0 > 0.0f;  // rows of a greedy request need the index of the maximum, the others the sum
   // exp(x / T) = 2^(x c); above 0, so that -infinity keeps its weight 0 where T is infinite
   const float c = sums ? fmaxf(fminf(1.44269504088896341f / T0, FLT_MAX), FLT_MIN) : 0.0f;
@@ -281,7 +292,13 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, i
   __shared__ int first;
   const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = a.row_off[r], hi = a.row_off[r + 1];
-  const bool valid = lo >= r && hi > lo && hi <= a.n_rows && hi - 1 - r <= a.n_rows - a.n_req;
+  // refused too: a request with drafts (which implies: or rows) that an earlier one has
+  bool over = !rows_fit(a, r, lo, hi);
+  for (int e = tid; e < r && !over; e += kDrawThreads) {
+    const int lo_e = a.row_off[e], hi_e = a.row_off[e + 1];
+    over = rows_fit(a, e, lo_e, hi_e) && hi_e - 1 - e > lo - r;
+  }
+  const bool valid = !__syncthreads_or(over);
   const float temp = a.temperature[r];
   if (tid < 16) tab[tid] = kSixteenths[tid];
   const bool writer = blockIdx.x == 0;

@@ -401,3 +401,33 @@ def test_verify_many_requests_and_graph(mk, torch_cuda):
         torch.cuda.synchronize()
         want = ref.verify(as64(lg), off, draft, q.numpy(), temp, u)
         check_verify((n_acc.cpu().numpy(), nxt.cpu().numpy(), p.cpu().numpy(), 0), want, len(draft))
+
+
+@pytest.mark.parametrize("R,rows,off,same,bad", [
+    (3, 6, [0, 9, 4, 6], [0, 2, 4, 6], [0, 1]),    # the first two leave the rows, the third stands by itself
+    (3, 6, [0, 2, -1, 6], [0, 2, 4, 6], [1, 2]),   # rows of the first behind which two bad ends lie
+    (3, 6, [3, 1, 4, 6], [0, 1, 4, 6], [0]),
+    (3, 8, [2, 6, 3, 7], [2, 6, 7, 8], [1, 2]),    # the third over the first's rows
+    (4, 9, [0, 3, 3, 6, 9], [0, 3, 4, 6, 9], [1, 2])])  # an empty request: the third's drafts would be the first's
+def test_verify_bad_tables_leave_the_others(mk, torch_cuda, R, rows, off, same, bad):
+    """Requests whose own rows are right keep their results, each with its own temperature, whatever stands beside them;
+    a request over an earlier one's rows or drafts is refused. `same`: a right table in which the others have the same rows."""
+    torch = torch_cuda
+    V = 500
+    for seed in range(6):
+        g = torch.Generator().manual_seed(seed)
+        lg = (torch.randn(rows, V, generator=g) * 2).cuda()
+        u = torch.rand(rows, generator=g, dtype=torch.float64).numpy()
+        draft = torch.randint(0, V, (rows - R,), generator=g).numpy()
+        temp = [[1.0, 0.0, 0.7, 2.5], [0.0, 0.9, 1.3, 0.0], [3.0, 0.5, 0.0, 1.0]][seed % 3][:R]
+        good = verify_call(mk, torch, F32, lg, V, same, draft, None, 0, temp, u, V, R)
+        assert good[3] == 0
+        got = verify_call(mk, torch, F32, lg, V, off, draft, None, 0, temp, u, V, R)
+        assert got[3] == mk.MK_ERR_ARG
+        for r in range(R):
+            if r in bad:
+                assert got[0][r] == 0 and got[1][r] == -1, (seed, r, got)
+            else:
+                assert got[0][r] == good[0][r] and got[1][r] == good[1][r], (seed, r, got, good)
+                js = slice(off[r] - r, off[r + 1] - 1 - r)
+                assert np.array_equal(got[2][js], good[2][js]), (seed, r)
