@@ -187,12 +187,13 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_verify_rows(VerifyArgs a, in
   }
 }
 
-// 2^t for -1000 < t <= 0 in 64 bits: t = n + k / 16 + f with |f| <= 1/32, 2^(k/16) from a table of 16 (one row of shared
-// memory's banks), the Taylor series of 2^f to degree 5 (remainder (ln 2 / 32)^6 / 6! = 1.4e-13), n into the exponent.
-__device__ __forceinline__ double exp2_64(double t, const double* tab) {
+// 2^t, t = x c, for -1000 < t <= 0 in 64 bits: t = n + k / 16 + f with |f| <= 1/32, 2^(k/16) from a table of 16 (one row of
+// shared memory's banks), the Taylor series of 2^f to degree 5 (remainder (ln 2 / 32)^6 / 6! = 1.4e-13), n into the exponent.
+// The product is fused into its two uses by name: every kernel that forms a weight has to round it alike.
+__device__ __forceinline__ double exp2_64(double x, double c, const double* tab) {
   constexpr double kRound = 6755399441055744.0 / 16;  // 1.5 * 2^48: adding it leaves round(16 t) in the low word
-  const double m = t + kRound;
-  const double f = t - (m - kRound);
+  const double m = fma(x, c, kRound);
+  const double f = fma(x, c, kRound - m);
   const int q = __double2loint(m);
   constexpr double L = 0.693147180559945309417;
   constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5;
@@ -206,8 +207,8 @@ __device__ __forceinline__ double exp2_64(double t, const double* tab) {
 }
 // exp((x - mx) / T) in 64 bits with c = log2 e / T: 0 for -infinity, NaN and what is below 2^-1000.
 __device__ __forceinline__ double weigh64(float x, float mx, double c, const double* tab) {
-  const double t = (static_cast<double>(fmaxf(x, -INFINITY)) - static_cast<double>(mx)) * c;
-  return t > -1000.0 ? exp2_64(t, tab) : 0.0;
+  const double d = static_cast<double>(fmaxf(x, -INFINITY)) - static_cast<double>(mx);
+  return d * c > -1000.0 ? exp2_64(d, c, tab) : 0.0;
 }
 __constant__ double kSixteenths[16] = {  // 2^(k/16)
     1.0, 1.0442737824274138403, 1.0905077326652576592, 1.1387886347566916537, 1.1892071150027210667,
@@ -259,7 +260,7 @@ struct Weigh {
         dense(d.draft >= 0 && with_q), token(d.draft >= 0 && !with_q ? d.token : -1) {}
   __device__ __forceinline__ double whole(float x) const {
     const bool some = (x - mx) * cf > -1000.0f;  // selected, not branched on: the chains of several calls interleave
-    const double y = exp2_64((static_cast<double>(some ? x : mx) - mx64) * c, tab);
+    const double y = exp2_64(static_cast<double>(some ? x : mx) - mx64, c, tab);
     return some ? y : 0.0;
   }
   __device__ __forceinline__ double rest(int j, float x, float q) const {
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, i
 
 template <typename T>
 __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_rest(VerifyArgs a, const Decision* decide, const double* zpart,
-                                                              double* rpart) {
+                                                              double* rpart, double* zsum) {
   __shared__ double tab[16], part[kDrawThreads / 32];
   const int r = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
   if (tid < 16) tab[tid] = kSixteenths[tid];
@@ -412,6 +413,7 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_rest(VerifyArgs a, c
   double z = 0.0;
   for (unsigned i = tid; i < gridDim.x; i += kDrawThreads) z += zpart[static_cast<int64_t>(r) * gridDim.x + i];
   w.Z = block_sum(z, part);
+  if (chunk == 0 && tid == 0) zsum[r] = w.Z;  // the pick takes this one: a sum in another order could move a residual's sign
   double v = 0.0;
 #pragma unroll
   for (int g = 0; g < kDrawVals; ++g) v += w.rest(chunk * kDrawChunk + g * kDrawThreads + tid, to_float(x[g]), y[g]);
@@ -448,7 +450,7 @@ __device__ __forceinline__ int reach(const double* p, int n, double target, int 
 
 template <typename T>
 __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a, const Decision* decide, const double* zpart,
-                                                              const double* rpart, int chunks) {
+                                                              const double* rpart, const double* zsum, int chunks) {
   __shared__ double tab[16], part[2][kPickWarps], seg[kPickWarps];
   const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < 16) tab[tid] = kSixteenths[tid];
@@ -458,6 +460,7 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a, cons
   const T* l = static_cast<const T*>(a.logits) + static_cast<int64_t>(d.row) * a.ld;
   const double* zp = zpart + static_cast<int64_t>(r) * chunks;
   const double* rp = rpart + static_cast<int64_t>(r) * chunks;
+  const double zs = d.draft >= 0 ? zsum[r] : 0.0;
   double z = 0.0, t = 0.0;
   for (int i = tid; i < chunks; i += kPickThreads) {
     z += zp[i];
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a, cons
   if (d.draft >= 0 && !(t > 0.0)) d.draft = -1;  // p <= q everywhere: draw from p
   const float* q = d.draft >= 0 && a.q ? a.q + static_cast<int64_t>(d.draft) * a.q_ld : nullptr;
   Weigh w(d, tab, q != nullptr);
-  w.Z = z;
+  w.Z = zs;
   const double target = d.u * (d.draft >= 0 ? t : z);
   // every warp finds the chunk; then the chunk's segments, one a warp, the segment's lanes and the lane's values
   double before = 0.0;
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(kPickThreads) k_verify_pick(VerifyArgs a, cons
 
 struct VerifyWs {
   int64_t chunks;  // of the draw
-  int64_t parts, decide, zpart, rpart, bytes;
+  int64_t parts, decide, zpart, rpart, zsum, bytes;
 };
 VerifyWs verify_ws(int n_rows, int n_req, int V) {
   VerifyWs w;
@@ -535,6 +538,7 @@ VerifyWs verify_ws(int n_rows, int n_req, int V) {
   w.decide = take(n_req * static_cast<int64_t>(sizeof(Decision)));
   w.zpart = take(n_req * w.chunks * 8);
   w.rpart = take(n_req * w.chunks * 8);
+  w.zsum = take(n_req * static_cast<int64_t>(8));
   w.bytes = std::max<int64_t>(at, 256);
   return w;
 }
@@ -550,6 +554,7 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
   Decision* decide = reinterpret_cast<Decision*>(p + y.decide);
   double* zpart = reinterpret_cast<double*>(p + y.zpart);
   double* rpart = reinterpret_cast<double*>(p + y.rpart);
+  double* zsum = reinterpret_cast<double*>(p + y.zsum);
   k_verify_rows<T><<<dim3(static_cast<unsigned>(a.n_rows), static_cast<unsigned>(n_chunks)), kRowThreads, 0, s>>>(
       a, tiles, n_chunks, parts);
   cudaError_t e = cudaGetLastError();
@@ -562,11 +567,11 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
                    decide, zpart, static_cast<int>(y.chunks), per);
   if (e == cudaSuccess)
     e = launch_pdl(k_verify_rest<T>, grid, dim3(kDrawThreads), 0, s, 1, a, static_cast<const Decision*>(decide),
-                   static_cast<const double*>(zpart), rpart);
+                   static_cast<const double*>(zpart), rpart, zsum);
   if (e == cudaSuccess)
     e = launch_pdl(k_verify_pick<T>, dim3(static_cast<unsigned>(a.n_req)), dim3(kPickThreads), 0, s, 1, a,
                    static_cast<const Decision*>(decide), static_cast<const double*>(zpart),
-                   static_cast<const double*>(rpart), static_cast<int>(y.chunks));
+                   static_cast<const double*>(rpart), static_cast<const double*>(zsum), static_cast<int>(y.chunks));
   return e;
 }
 

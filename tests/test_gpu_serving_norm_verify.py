@@ -431,3 +431,23 @@ def test_verify_bad_tables_leave_the_others(mk, torch_cuda, R, rows, off, same, 
                 assert got[0][r] == good[0][r] and got[1][r] == good[1][r], (seed, r, got, good)
                 js = slice(off[r] - r, off[r + 1] - 1 - r)
                 assert np.array_equal(got[2][js], good[2][js]), (seed, r)
+
+
+def test_verify_residual_of_one_rounding(mk, torch_cuda):
+    """One entry of the residual is above 0, by less than a rounding of the row's sum: found by trying temperatures until
+    p - q had that sign for the sum of the 384 chunks' shares taken 256 at a time, and the other one taken 512 at a time. The
+    token drawn is that entry, since the sum behind the residual's total is also the one behind the draw."""
+    torch = torch_cuda
+    chunks, size, temp, seed = 384, 4096, 1.88917732, 2076039816
+    V = chunks * size
+    lg = torch.full((2, V), -float("inf"))
+    s, classes = 2 * seed + 1, []
+    for i in range(chunks):  # one token a chunk, 0, 1, 2 or 4 below the first
+        s = (s * 6364136223846793005 + 1442695040888963407) % 2 ** 64
+        classes.append(0 if i == 0 else (s >> 40) & 3)
+        lg[:, i * size + 17] = -[0.0, 1.0, 2.0, 4.0][classes[-1]]
+    token = classes.index(3) * size + 17
+    q = torch.ones(1, V)
+    q[0, token] = 0.000591546181
+    got = verify_call(mk, torch, F32, lg.cuda(), V, [0, 2], [17], q.cuda(), V, [temp], [0.99, 0.5], V, 1)
+    assert got[0][0] == 0 and got[1][0] == token and got[3] == 0, got
