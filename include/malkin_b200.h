@@ -412,11 +412,13 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
  * running sum in index order reaches u x the total. temperature <= 0 (or NaN): kept while it is the row's argmax (the
  * lowest index of the maximum), next = argmax; dev_q and the uniforms are not used.
  * Results: dev_n_acc[r] drafts kept, dev_next[r], dev_p[x - r] (NULL: not wanted) the target's probability of each draft
- * looked at, 0 for those after the first one that was not kept. A draft outside 0 .. V - 1 has probability 0. Logits of
- * -infinity are tokens that cannot be drawn, NaN logits count as -infinity; a row whose maximum is not finite has no
- * distribution: no draft is kept on it, and as the row drawn from it gives dev_next = -1. A request whose rows are not as
- * above, or that has rows or drafts of an earlier one whose rows are in the buffers, gives dev_n_acc = 0, dev_next = -1 and
- * records MK_ERR_ARG (its dev_p entries are not written); the others are not changed by it.
+ * looked at, 0 for those after the first one that was not kept. It comes from a row sum of 32-bit exponentials: within
+ * 2^-16 of itself, 2^-23 as a rule. What is decided (kept or not, the token drawn) follows 64-bit sums to some 10^-13. A
+ * draft outside 0 .. V - 1 has probability 0. Logits of -infinity are tokens that cannot be drawn, NaN logits count as
+ * -infinity; a row whose maximum is not finite has no distribution: no draft is kept on it, and as the row drawn from it
+ * gives dev_next = -1. A request whose rows are not as above, or that has rows or drafts of an earlier one whose rows are
+ * in the buffers, gives dev_n_acc = 0, dev_next = -1 and records MK_ERR_ARG (its dev_p entries are not written); the others
+ * are not changed by it.
  * dev_ws: mk_verify_draft_workspace(n_rows, n_req, V) bytes, 16-byte aligned. V at most 2^27, n_req at most 65535. */
 int64_t mk_verify_draft_workspace(int n_rows, int n_req, int V);
 int mk_verify_draft(int type, const void* dev_logits, int64_t ld, int n_rows, int V, int n_req,

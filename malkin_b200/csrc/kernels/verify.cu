@@ -13,9 +13,10 @@
 //                  draw needs
 //   k_verify_rest  CTAs (request, chunk): the chunk's share of the draw's total
 //   k_verify_pick  one CTA per request: the chunk, the segment and the token the running sum reaches its target in
-// A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the
+// A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the drawn
 // row's exponentials and sums are in 64 bits: with 32 the drawn index would differ from the exact one about once in 10^4
-// draws. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
+// draws. An acceptance compares with one probability: its exponential is in 64 bits, its row's sum is k_verify_rows' of 32-bit
+// exponentials (off by 8e-8 of itself as a rule), and where that could decide, the row is summed again in 64 bits. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
 // slower: 93, 85 and 96 us against 75 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
 // Measured, V = 151936: 64 requests of 5 fp32 rows with probabilities 75 to 78 us, of which k_verify_rows 35 (5.6 TB/s, 0.85 of
 // a copy's rate); one request of 9 fp32 rows 19 us, 8 requests of up to 9 bf16 rows 24, both held by four dependent launches.
@@ -285,14 +286,22 @@ __device__ __forceinline__ void load_chunk(const T* row, int chunk, int V, T fil
   }
 }
 
+// Where u q(d) lies this near p(d), relative to it, the row's sum is formed again in 64 bits. The sum behind p is of 32-bit
+// exponentials 2^t and off by less than 120 x 2^-23 < 2^-16 of itself for rows of up to 2^27 tokens: t carries three roundings,
+// 1.5 x 2^-23 |t| ln 2 of a weight, and the mean of |t| under the weights is at most log2 V = 27 (28); 2^x is good to 2^-22 (2);
+// a thread adds at most 128 weights (64) and brings them to a larger maximum at most 8 times, its block and warp once (25).
+constexpr double kClose = 1.0 / (1 << 15);
+
 // Grid: (CTAs of a request, request); each takes `per` of the draw's chunks.
 template <typename T>
 __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, int n_chunks, const RowPart* parts,
                                                               Decision* decide, double* zpart, int chunks, int per) {
   __shared__ double tab[16], part[kDrawThreads / 32];
-  __shared__ int first;
+  __shared__ int first, close;  // draft that is not kept, that is too close to tell; `last`: none
+  __shared__ int from, last;    // drafts before `from` are kept, that at `last` is not (k: none)
   const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = a.row_off[r], hi = a.row_off[r + 1];
+  const float temp = a.temperature[r];
   // refused too: a request with drafts (which implies: or rows) that an earlier one has
   bool over = !rows_fit(a, r, lo, hi);
   for (int e = tid; e < r && !over; e += kDrawThreads) {
@@ -300,7 +309,6 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, i
     over = rows_fit(a, e, lo_e, hi_e) && hi_e - 1 - e > lo - r;
   }
   const bool valid = !__syncthreads_or(over);
-  const float temp = a.temperature[r];
   if (tid < 16) tab[tid] = kSixteenths[tid];
   const bool writer = blockIdx.x == 0;
   pdl_launch();
@@ -318,77 +326,102 @@ __global__ void __launch_bounds__(kDrawThreads, 4) k_verify_norm(VerifyArgs a, i
   const bool greedy = !(temp > 0.0f);
   const double c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temp);
   const T* logits = static_cast<const T*>(a.logits);
-  if (tid == 0) first = k;
+  const int c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
+  // Once around as a rule. A draft that is too close to tell takes a turn of its own, in which every CTA forms the whole sum of
+  // its row by the code that forms the chunks' shares (a second copy of that code costs 0.7 us a call without being reached, this
+  // 0.3 to 0.9).
+  if (tid == 0) from = 0, first = close = last = k;
   __syncthreads();
   pdl_wait();
-  for (int i = warp; i < k; i += kDrawThreads / 32) {
-    const int d = a.draft[j0 + i];
-    const bool in = d >= 0 && d < a.V;
-    float l = -INFINITY, qd = 0.0f;
-    if (in && !greedy) {
-      l = to_float(logits[static_cast<int64_t>(lo + i) * a.ld + d]);
-      qd = a.q ? a.q[static_cast<int64_t>(j0 + i) * a.q_ld + d] : 1.0f;
-    }
-    const double ui = a.u[lo + i];
-    float mx;
-    int idx;
-    double sum;
-    join_row(parts + static_cast<int64_t>(lo + i) * n_chunks, n_chunks, c, tab, lane, mx, idx, sum);
-    if (lane == 0) {
-      const bool some = mx > -INFINITY && mx < INFINITY;
-      double p = 0.0;
-      bool keep;
-      if (greedy) {
-        p = some && d == idx ? 1.0 : 0.0;
-        keep = p > 0.0;
-      } else {
-        if (some) p = weigh64(l, mx, c, tab) / sum;
-        keep = qd > 0.0f && ui * static_cast<double>(qd) < p;
+  for (;;) {
+    for (int i = from + warp; i < last; i += kDrawThreads / 32) {
+      const int d = a.draft[j0 + i];
+      const bool in = d >= 0 && d < a.V;
+      float l = -INFINITY, qd = 0.0f;
+      if (in && !greedy) {
+        l = to_float(logits[static_cast<int64_t>(lo + i) * a.ld + d]);
+        qd = a.q ? a.q[static_cast<int64_t>(j0 + i) * a.q_ld + d] : 1.0f;
       }
-      if (!keep) atomicMin(&first, i);
-      if (writer && a.p) a.p[j0 + i] = static_cast<float>(p);
+      const double ui = a.u[lo + i];
+      float mx;
+      int idx;
+      double sum;
+      join_row(parts + static_cast<int64_t>(lo + i) * n_chunks, n_chunks, c, tab, lane, mx, idx, sum);
+      if (lane == 0) {
+        const bool some = mx > -INFINITY && mx < INFINITY;
+        double p = 0.0;
+        bool keep, near = false;
+        if (greedy) {
+          p = some && d == idx ? 1.0 : 0.0;
+          keep = p > 0.0;
+        } else {
+          if (some) p = weigh64(l, mx, c, tab) / sum;
+          const double uq = ui * static_cast<double>(qd);
+          keep = qd > 0.0f && uq < p;
+          near = qd > 0.0f && p > 0.0 && fabs(uq - p) <= kClose * p;
+        }
+        if (near)
+          atomicMin(&close, i);
+        else if (!keep)
+          atomicMin(&first, i);
+        if (writer && a.p) a.p[j0 + i] = static_cast<float>(p);
+      }
     }
-  }
-  __syncthreads();
-  const int stop = first, row = lo + stop;
-  if (writer) {
-    if (a.p)
-      for (int i = stop + 1 + tid; i < k; i += kDrawThreads) a.p[j0 + i] = 0.0f;  // never looked at
-    if (tid == 0) a.n_acc[r] = stop;
-  }
-  Decision d;
-  int idx;
-  double unused;
-  join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, tab, lane, d.mx, idx, unused);
-  const bool some = d.mx > -INFINITY && d.mx < INFINITY;
-  d.draw = some && !greedy;
-  d.row = row;
-  d.draft = stop < k ? j0 + stop : -1;
-  d.token = stop < k ? a.draft[j0 + stop] : -1;
-  d.c = c;
-  d.u = a.u[row + (stop < k ? 1 : 0)];
-  d.pad = 0.0f;
-  if (writer && tid == 0) {
-    decide[r] = d;
-    if (!d.draw) a.next[r] = some ? idx : -1;
-  }
-  if (!d.draw) return;
-  const T* l = logits + static_cast<int64_t>(row) * a.ld;
-  const Weigh w(d, tab, a.q != nullptr);
-  T next[kDrawVals];
-  auto load = [&](int chunk) { load_chunk(l, chunk, a.V, from_float<T>(-INFINITY), next); };
-  const int c0 = blockIdx.x * per, c1 = min(chunks, c0 + per);
-  load(c0);
-  for (int chunk = c0; chunk < c1; ++chunk) {
-    float x[kDrawVals];
-#pragma unroll
-    for (int g = 0; g < kDrawVals; ++g) x[g] = to_float(next[g]);
-    if (chunk + 1 < c1) load(chunk + 1);
+    __syncthreads();
+    const int stop = min(first, close), row = lo + stop;
+    const bool settle = close < first;
+    Decision d;
+    int idx;
+    double unused;
+    join_row(parts + static_cast<int64_t>(row) * n_chunks, n_chunks, c, tab, lane, d.mx, idx, unused);
+    const bool some = d.mx > -INFINITY && d.mx < INFINITY;
+    d.draw = some && !greedy;
+    d.row = row;
+    d.draft = stop < k ? j0 + stop : -1;
+    d.token = stop < k ? a.draft[j0 + stop] : -1;
+    d.c = c;
+    d.u = a.u[row + (stop < k ? 1 : 0)];
+    d.pad = 0.0f;
+    if (writer && !settle) {
+      if (a.p)
+        for (int i = stop + 1 + tid; i < k; i += kDrawThreads) a.p[j0 + i] = 0.0f;  // never looked at
+      if (tid == 0) {
+        a.n_acc[r] = stop;
+        decide[r] = d;
+        if (!d.draw) a.next[r] = some ? idx : -1;
+      }
+    }
+    if (!d.draw) return;
+    const T* l = logits + static_cast<int64_t>(row) * a.ld;
+    const Weigh w(d, tab, a.q != nullptr);
+    T next[kDrawVals];
+    auto load = [&](int chunk) { load_chunk(l, chunk, a.V, from_float<T>(-INFINITY), next); };
+    const int end = settle ? chunks : c1;
     double v = 0.0;
+    load(settle ? 0 : c0);
+    for (int chunk = settle ? 0 : c0; chunk < end; ++chunk) {
+      float x[kDrawVals];
 #pragma unroll
-    for (int g = 0; g < kDrawVals; ++g) v += w.whole(x[g]);
-    v = block_sum(v, part);
-    if (tid == 0) zpart[static_cast<int64_t>(r) * chunks + chunk] = v;
+      for (int g = 0; g < kDrawVals; ++g) x[g] = to_float(next[g]);
+      if (chunk + 1 < end) load(chunk + 1);
+#pragma unroll
+      for (int g = 0; g < kDrawVals; ++g) v += w.whole(x[g]);
+      if (settle) continue;
+      v = block_sum(v, part);
+      if (tid == 0) zpart[static_cast<int64_t>(r) * chunks + chunk] = v;
+      v = 0.0;
+    }
+    if (!settle) return;
+    // a draft that is too close has a token and a q above 0
+    const double p = w.whole(to_float(l[d.token])) / block_sum(v, part);
+    const double uq = a.u[row] * static_cast<double>(a.q ? a.q[static_cast<int64_t>(d.draft) * a.q_ld + d.token] : 1.0f);
+    if (writer && a.p && tid == 0) a.p[d.draft] = static_cast<float>(p);
+    if (tid == 0) {  // block_sum's barriers lie behind the last use of these
+      from = uq < p ? stop + 1 : stop;
+      if (!(uq < p)) last = stop;
+      first = close = last;
+    }
+    __syncthreads();
   }
 }
 

@@ -451,3 +451,33 @@ def test_verify_residual_of_one_rounding(mk, torch_cuda):
     q[0, token] = 0.000591546181
     got = verify_call(mk, torch, F32, lg.cuda(), V, [0, 2], [17], q.cuda(), V, [temp], [0.99, 0.5], V, 1)
     assert got[0][0] == 0 and got[1][0] == token and got[3] == 0, got
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("V,with_q", [(700, True), (30011, True), (151936, False)])
+def test_verify_at_the_border(mk, torch_cuda, t, V, with_q):
+    """u q(d) a part in 10^11 below and above p(d): the acceptance is that of the 64-bit rule, one draft or several in a
+    row (both sides' sums are good to some 10^-13)."""
+    torch = torch_cuda
+    R, K = 24, 3
+    g = torch.Generator().manual_seed(V)
+    lg = (torch.randn(R * (K + 1), V, generator=g) * 1.5).to(torch_type(torch, t)).cuda()
+    x = as64(lg)
+    temp = (0.6 + 0.05 * np.arange(R)).astype(np.float32)
+    off = np.arange(R + 1) * (K + 1)
+    draft, u = np.zeros(R * K, np.int64), np.full(R * (K + 1), 0.4)
+    q = np.full((R * K, V), 0.5 / V, np.float32)
+    stop = [r % (K + 1) for r in range(R)]  # the draft that is refused; K: none
+    for r in range(R):
+        for i in range(K):
+            p = ref.softmax(x[off[r] + i] / np.float64(temp[r]))
+            d = int(np.argsort(-p)[3 + i])
+            draft[r * K + i] = d
+            q[r * K + i, d] = 1.25 * p[d]
+            qd = float(q[r * K + i, d]) if with_q else 1.0
+            u[off[r] + i] = p[d] / qd * (1 + 1e-11 if i >= stop[r] else 1 - 1e-11)
+    qd = torch.as_tensor(q).cuda() if with_q else None
+    got = verify_call(mk, torch, t, lg, V, off, draft, qd, V, temp, u, V, R)
+    want = ref.verify(x, off, draft, q if with_q else None, temp, u)
+    assert list(want[0]) == stop
+    check_verify(got, want, len(draft))
