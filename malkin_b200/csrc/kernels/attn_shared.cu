@@ -14,14 +14,17 @@
 //
 // int8 values are exact in both 16-bit types. Row scales of K (with scale and log2 e) multiply the scores, those of V the
 // weights. P V is in fp16 whatever q's type: a weight x scale is rounded by 2^-11 of itself (bf16 would lose 2^-8, which is
-// what an fp16 output would then be off by). To stay in fp16's range the row's reference exponent is not the largest score
-// but that plus the exponent of the block's largest V scale, less 6: products are at most 2^15, and full precision reaches
-// down to 2^-20 of the largest. Sums and outputs carry the same reference, so it cancels.
+// what an fp16 output would then be off by). To stay in fp16's range a row's reference exponent is not its largest score but the
+// largest sum of a score and the exponent of that key's V scale, over the keys the row sees, less 6: products are at most 2^15,
+// and full precision reaches down to 2^-20 of the row's largest. Sums and outputs carry the same reference, so it cancels. Where
+// the scales of a block lie within 2^4 of each other, as they do as a rule, the largest stands for each of them: that costs at
+// most 4 of those 20 bits and spares the sums (two prefixes of 32768 rows: 257 us, with the sums in every block 263; the block's
+// largest scale alone, seen by the row or not, 246, and wrong where scales lie far apart).
 // Bound: HBM for one tile of rows a group (128 rows: 65.5 kFLOP against 264 bytes a key and head, the machine's balance),
 // the tensor pipe and the conversion above that. What holds it: a block of 96 keys takes 3700 cycles for 128 rows and 3900 for
 // 256, 2500 of them the widening (K to bf16 1700, V to fp16 800); the plan takes 7 us, finding a piece's place 2, the join 4 to
 // 5. Measured, with queries of 32 / 8 heads of 128: two prefixes of up to 32768 rows with 32 requests of 4 rows each, bf16:
-// 246 to 252 us; 8 trees of 17 rows behind 2048 rows, fp16: 44; 4 single rows behind 1000, 16 / 8 heads, bf16: 25. Two CTAs an
+// 257 us; 8 trees of 17 rows behind 2048 rows, fp16: 44; 4 single rows behind 1000, 16 / 8 heads, bf16: 25. Two CTAs an
 // SM with blocks of 64 keys took 497 us at the first.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -51,7 +54,8 @@ constexpr int kAttendThreads = 512;  // warpgroups: softmax of stream 0, of stre
 constexpr int kRegsSoftmax = 176, kRegsConvert = 80, kRegsMma = 80;  // 2 x 176 + 80 + 80 = 4 x the 128 of the launch
 constexpr float kRaiseMax = 8.0f;   // a row's reference is raised when it is to grow by more (exponents of 2)
 constexpr float kHeadroom = 6.0f;   // of it below the largest weight x scale
-constexpr int kLeastExp = -40;      // of a block's largest V scale: blocks of zeros must not push the sums out of range
+constexpr int kLeastExp = -40;      // of a V scale: rows of zeros must not push the sums out of range
+constexpr int kSpread = 4;          // of a block's exponents, to be taken for one
 
 // Tokens and keys of a unit (with a KV head). Its places on the line: one for each block (a block takes about as long for
 // 256 rows as for 128: 3900 and 3700 cycles), after `open` for what a part costs before its first block and after its last.
@@ -386,6 +390,11 @@ struct Walk {
   }
 };
 
+// Exponent of a V scale.
+__device__ __forceinline__ float exponent(float v) {
+  return static_cast<float>(max(static_cast<int>(__float_as_uint(fabsf(v)) >> 23) - 127, kLeastExp));
+}
+
 // ---------------- int8 to 16-bit ----------------
 // 4 int8 values -> two words of two 16-bit values, exact.
 template <typename T>
@@ -433,14 +442,14 @@ struct SharedSmall {
   uint64_t q_full[2], q_empty[2], full[5], empty[5], raw_full[3], raw_empty[3], s_full[2], p_full[2], pv_done[2], o_free[2], b_fin;
   alignas(16) float ks[kScaleSlots][kBlock];  // K scale x scale x log2 e
   alignas(16) float vs[kScaleSlots][kBlock];
-  alignas(16) float vmax[kScaleSlots][4];     // largest finite |V scale| of each 32 keys of the block
+  alignas(16) int hi[kScaleSlots][4], lo[kScaleSlots][4];  // exponent fields of each 32 keys' V scales: largest, least above 0
   uint32_t odd[kScaleSlots][4];   // those whose V scale is not finite, a bit each (the scale is kept as 0)
   Part part[kParts];
   float2 ml[kTileRows];           // stream 1's reference and sum, for stream 0 where they share the rows
   uint32_t tmem;
 };
 static_assert(offsetof(SharedSmall, ks) % 16 == 0 && offsetof(SharedSmall, vs) % 16 == 0 &&
-                  offsetof(SharedSmall, vmax) % 16 == 0 && sizeof(float) * kBlock % 16 == 0,
+                  offsetof(SharedSmall, hi) % 16 == 0 && offsetof(SharedSmall, lo) % 16 == 0 && sizeof(float) * kBlock % 16 == 0,
               "scales are read as 16-byte words");
 template <int D>
 constexpr int shared_smem() {
@@ -562,18 +571,26 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(const __gri
             for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const float4 vm = *reinterpret_cast<const float4*>(sm->vmax[sl]);
-          const float big = fmaxf(fmaxf(vm.x, vm.y), vm.z);
+          const int4 hi = *reinterpret_cast<const int4*>(sm->hi[sl]), lo = *reinterpret_cast<const int4*>(sm->lo[sl]);
+          const int most = max(max(hi.x, hi.y), hi.z), least = min(min(lo.x, lo.y), lo.z);
+          float want = top + static_cast<float>(max(most - 127, kLeastExp));
           const uint32_t* odd = sm->odd[sl];
-          if (odd[0] | odd[1] | odd[2]) {
+          if (odd[0] | odd[1] | odd[2] | static_cast<uint32_t>(most - least > kSpread)) {  // one branch for what is rare
 #pragma unroll 1
             for (int i = 0; i < 3; ++i) {
               const int v = left - 32 * i;
               spoilt |= (odd[i] & (v >= 32 ? 0xFFFFFFFFu : v <= 0 ? 0u : (1u << v) - 1)) != 0;
             }
+            // exponents shuffled from a lane's three keys (loaded one by one: 46 us for 44, 8 trees)
+            const float e0 = exponent(sm->vs[sl][lane]), e1 = exponent(sm->vs[sl][32 + lane]), e2 = exponent(sm->vs[sl][64 + lane]);
+            want = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              want = max3(want, x[i] + __shfl_sync(0xffffffffu, e0, i), x[32 + i] + __shfl_sync(0xffffffffu, e1, i));
+              want = fmaxf(want, x[64 + i] + __shfl_sync(0xffffffffu, e2, i));
+            }
           }
-          const int e = max(static_cast<int>(__float_as_uint(big) >> 23) - 127, kLeastExp);
-          const float want = top + (static_cast<float>(e) - kHeadroom);
+          want -= kHeadroom;
           float scale = 1.0f;
           if (want > m && (m == -INFINITY || want - m > kRaiseMax)) {
             scale = ex2_approx(m - want);
@@ -755,11 +772,12 @@ __global__ void __launch_bounds__(kAttendThreads, 1) k_shared_attend(const __gri
       if (!ready(2 * gb)) break;
       if (t < kBlock) {
         const bool fine = fabsf(vs) < INFINITY;
-        const float big = warp_max(fine ? fabsf(vs) : 0.0f);
+        const int e = fine ? static_cast<int>(__float_as_uint(fabsf(vs)) >> 23) : 0;
+        const int hi = __reduce_max_sync(0xffffffffu, e), lo = __reduce_min_sync(0xffffffffu, e ? e : 255);
         const uint32_t odd = __ballot_sync(0xffffffffu, !fine);
         sm->ks[sl][t] = ks * kscale;
         sm->vs[sl][t] = fine ? vs : 0.0f;
-        if (lane == 0) sm->vmax[sl][t >> 5] = big, sm->odd[sl][t >> 5] = odd;
+        if (lane == 0) sm->hi[sl][t >> 5] = hi, sm->lo[sl][t >> 5] = lo, sm->odd[sl][t >> 5] = odd;
       }
       if (++b == end) open();
       if (!ok) break;

@@ -314,3 +314,39 @@ def test_agrees_with_the_exact_attention(mk, torch_cuda):
     want = out.cpu().numpy()
     # both within their own error of the exact value; |v| <= 2.6 here
     assert np.abs(got - want).max() <= (W_PART + 2.0 ** -11) * 2.6
+
+
+@pytest.mark.parametrize("value", [1e30, 1e12, -1e30])
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_v_scales_of_keys_a_row_does_not_see(mk, torch_cuda, t, value):
+    """A row of the cache that only later tokens of the request look at may have any finite scale."""
+    H, KV, D = 4, 2, 64
+    b = Batch(np.random.default_rng(3), [(100, [(20, 3), (5, "tree", 2)])], KV, D, 1)
+    q = queries(torch_cuda, t, b.n, H, D, 4)
+    b.vs[:, b.kv_base[0] + 21] = value  # the row that only the third token of the first request sees
+    got = call(mk, torch_cuda, t, b, q, H, KV, D)
+    check(torch_cuda, t, b, q, got, H, KV, D, tokens=[i for i in range(b.n) if i != 2])
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_v_scales_far_apart(mk, torch_cuda, t, D):
+    """Scales of V over many powers of two, the largest of them on keys of hardly any weight: no product that counts is
+    lost. (A product weight x scale is rounded by 2^-11 of itself or by 2^-31 of the row's largest in the block; with |v|
+    between 32 and 127 and 700 keys the latter stay below 700 x 4 x 2^-31 of sum w |v|.)"""
+    H, KV = 8, 2
+    for seed in range(3):
+        rng = np.random.default_rng(seed)
+        b = Batch(rng, [(500, [(40, 2), (90, "tree", 2), (200, 1)]), (0, [(97, 2)])], KV, D, 1)
+        b.v = (rng.integers(32, 128, b.v.shape) * rng.choice([-1, 1], b.v.shape)).astype(np.int8)
+        b.vs = (10.0 ** rng.uniform(-5, 2, b.vs.shape)).astype(np.float32)
+        q = queries(torch_cuda, t, b.n, H, D, seed)
+        # keys that every query is far from: scores some 40 below the others, V scales of 10^9
+        q[:, ::D] = 8.0
+        b.k[:, :, 0] = 0
+        far = rng.random(b.rows) < 0.03
+        b.k[:, far, 0] = -127
+        b.ks[:, far] = 40.0 * D ** 0.5 / (8 * 127)
+        b.k[:, far, 1:] = 0
+        b.vs[:, far] = 1e9
+        check(torch_cuda, t, b, q, call(mk, torch_cuda, t, b, q, H, KV, D), H, KV, D)
