@@ -1094,7 +1094,8 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
         for (int u = 0; u < 4; ++u) {
           if (u < some) {
             const float g = ex2_approx(s[u] - top);
-            l += g;
+            // a V scale that is not finite: the output is NaN, as where the row is a prefix or own one
+            l += fabsf(vs[u]) < INFINITY ? g : __int_as_float(0x7FFFFFFF);
 #pragma unroll
             for (int e = 0; e < N; ++e) o[e] += g * vs[u] * v[u][e];
           }

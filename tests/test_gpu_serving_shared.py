@@ -350,3 +350,21 @@ def test_v_scales_far_apart(mk, torch_cuda, t, D):
         b.k[:, far, 1:] = 0
         b.vs[:, far] = 1e9
         check(torch_cuda, t, b, q, call(mk, torch_cuda, t, b, q, H, KV, D), H, KV, D)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_ancestor_with_a_scale_that_is_not_finite(mk, torch_cuda, value):
+    """A V scale that is not finite makes the tokens NaN that have its row for an ancestor, as those that have it among
+    their own keys, and nobody else."""
+    torch = torch_cuda
+    H, KV, D = 4, 2, 64
+    b = Batch(np.random.default_rng(3), [(100, [(20, 3), (5, "tree", 3)])], KV, D, 1)
+    q = queries(torch, BF16, b.n, H, D, 4)
+    first = 3  # the tree's root token; its next two rows are its children
+    row = b.kv_base[first] + 5
+    b.vs[:, row] = value
+    hit = [i for i in range(b.n) if row in b.keys_of(i)]
+    assert 1 < len(hit) < b.n - 4
+    got = call(mk, torch, BF16, b, q, H, KV, D)
+    check(torch, BF16, b, q, got, H, KV, D, tokens=[i for i in range(b.n) if i not in hit])
+    assert np.isnan(got[hit, :H * D]).all()
