@@ -386,8 +386,9 @@ int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* d
  * 128, scale > 0; dev_q, dev_k, dev_v and dev_out 16-byte aligned, dev_ws 32-byte, strides multiples of 8. A scale of V that
  * is not finite makes the outputs of the tokens that see its row NaN.
  * Rows outside the tables are not looked at, nor are their scales. A group or token whose rows leave the cache, or a group
- * whose tokens leave 0 .. n, has none of those keys, a token whose ancestors do loses them from the first such one on, and
- * MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside a kernel ran out, the outputs are not valid.
+ * whose tokens leave 0 .. n or begin before the end of an earlier group, has none of those keys, a token whose ancestors do
+ * loses them from the first such one on, and MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside a kernel ran
+ * out, the outputs are not valid.
  * dev_ws: mk_attention_shared_workspace(n, H, KV, D, n_groups) bytes (negative: bad shape or no device): the
  * partial results, 4 (D + 2) bytes for each of 4 n H rows and of 256 rows a multiprocessor, and the tables of the plan. */
 int64_t mk_attention_shared_workspace(int n, int H, int KV, int D, int n_groups);

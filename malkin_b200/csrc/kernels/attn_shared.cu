@@ -144,7 +144,8 @@ __device__ __forceinline__ V block_scan_sum(V v, V* part, V& total) {  // inclus
   return v + (warp ? part[warp - 1] : V(0));
 }
 
-__device__ __forceinline__ int block_scan_max(int v, int* part) {  // inclusive
+// Inclusive, of values from 0 on; left: without the thread's own.
+__device__ __forceinline__ int block_scan_max(int v, int* part, int& left) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -164,7 +165,10 @@ __device__ __forceinline__ int block_scan_max(int v, int* part) {  // inclusive
     part[lane] = w;
   }
   __syncthreads();
-  return warp ? max(v, part[warp - 1]) : v;
+  const int before = warp ? part[warp - 1] : 0;
+  left = __shfl_up_sync(0xffffffffu, v, 1);
+  left = lane ? max(left, before) : before;
+  return max(v, before);
 }
 
 // Keys of the token in its own sequence, 0 when the table leaves the cache.
@@ -185,46 +189,55 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
   const int G = a.H / a.KV, half = kTileRows / G, per_tile = 2 * half;
   bool bad = false;
   for (int t = tid; t < a.n; t += kPlanThreads) w.tok_pre[t] = -1;
-  // prefix tiles
-  int n_tiles = 0;
-  for (int g0 = 0; g0 < a.n_groups; g0 += kPlanThreads) {
-    const int g = g0 + tid;
-    int lo = 0, hi = 0, base = 0, len = 0;
-    if (g < a.n_groups) {
-      lo = a.group_off[g];
-      hi = a.group_off[g + 1];
-      base = a.prefix_base[g];
-      len = a.prefix_len[g];
-      if (lo < 0 || hi < lo || hi > a.n || base < 0 || len < 0 || static_cast<int64_t>(base) + len > a.n_rows) {
-        bad = true;
-        lo = hi = len = 0;
+  // prefix tiles. A group that begins before the end of an earlier one is refused, so that a token is in one group at most and
+  // the tiles are no more than there is room for. Offsets that nowhere descend put no token into two groups: only where one is
+  // seen to, or there are several rounds of groups, the ends before each are looked at (`careful`, a second time around).
+  int n_tiles;
+  for (bool careful = a.n_groups > kPlanThreads;; careful = true) {
+    bool falls = false;
+    int grouped = 0;  // end of the groups before the round
+    n_tiles = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += kPlanThreads) {
+      const int g = g0 + tid;
+      int lo = 0, hi = 0, base = 0, len = 0;
+      if (g < a.n_groups) {
+        lo = a.group_off[g];
+        hi = a.group_off[g + 1];
+        base = a.prefix_base[g];
+        len = a.prefix_len[g];
+        falls = hi < lo;
+        if (lo < 0 || hi < lo || hi > a.n || base < 0 || len < 0 || static_cast<int64_t>(base) + len > a.n_rows) {
+          bad = true;
+          lo = hi = len = 0;
+        }
       }
-    }
-    const int tiles = len > 0 ? (hi - lo + per_tile - 1) / per_tile : 0;
-    int total;
-    const int first = n_tiles + block_scan_sum(tiles, part, total) - tiles;
-    if (g < a.n_groups) {
-      w.group_tile[g] = tiles > 0 ? first : -1;
-      for (int i = 0; i < tiles && first + i < w.prefix_tiles; ++i) {
-        Tile& x = w.tile[first + i];
-        x.t0 = lo + i * per_tile;
-        x.nt = min(per_tile, hi - x.t0);
-        x.base = base;
-        x.len = len;
-        x.own = 0;
+      if (careful) {
+        int before;
+        block_scan_max(hi > lo ? hi : 0, part, before);
+        if (hi > lo && lo < max(before, grouped)) {
+          bad = true;
+          hi = lo;
+        }
+        grouped = max(grouped, part[31]);
       }
+      const int tiles = len > 0 ? (hi - lo + per_tile - 1) / per_tile : 0;
+      int total;
+      const int first = n_tiles + block_scan_sum(tiles, part, total) - tiles;
+      if (g < a.n_groups) {
+        w.group_tile[g] = tiles > 0 ? first : -1;
+        for (int i = 0; i < tiles && first + i < w.prefix_tiles; ++i) {  // all of them, once no token is in two groups
+          Tile& x = w.tile[first + i];
+          x.t0 = lo + i * per_tile;
+          x.nt = min(per_tile, hi - x.t0);
+          x.base = base;
+          x.len = len;
+          x.own = 0;
+        }
+      }
+      n_tiles += total;  // at most 2^29 in a round that is not careful, which is the only one
     }
-    n_tiles = min(n_tiles + total, w.prefix_tiles + 1);  // a round adds at most 2^29
+    if (!__syncthreads_or(falls && !careful)) break;
   }
-  if (n_tiles > w.prefix_tiles) {  // groups that overlap one another: no result
-    for (int t = tid; t < a.n; t += kPlanThreads) w.tok_own[t] = -1;
-    if (tid == 0) {
-      *w.head = PlanHead{0, 1, 0, 0};
-      if (a.status) atomicCAS(a.status, 0, kStatusBadIndex);
-    }
-    return;
-  }
-  __syncthreads();
   for (int g = warp; g < a.n_groups; g += kPlanThreads / 32) {
     const int first = w.group_tile[g];
     if (first < 0) continue;
@@ -238,7 +251,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_shared_plan(SharedArgs a, Shar
     const int t = t0 + tid;
     const bool in = t < a.n;
     const bool start = in && (t == 0 || a.kv_base[t] != a.kv_base[t - 1]);
-    const int from = max(run, block_scan_max(start ? t : 0, part));
+    int left;
+    const int from = max(run, block_scan_max(start ? t : 0, part, left));
     const int cut = in && (t - from) % per_tile == 0 ? 1 : 0;
     int total;
     const int idx = n_tiles + block_scan_sum(cut, part, total) - 1;

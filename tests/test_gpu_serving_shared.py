@@ -368,3 +368,34 @@ def test_ancestor_with_a_scale_that_is_not_finite(mk, torch_cuda, value):
     got = call(mk, torch, BF16, b, q, H, KV, D)
     check(torch, BF16, b, q, got, H, KV, D, tokens=[i for i in range(b.n) if i not in hit])
     assert np.isnan(got[hit, :H * D]).all()
+
+
+@pytest.mark.parametrize("off", [[0, 4, 0, 7], [0, 4, 2, 6, 7], [0, 4, 4, 1, 4, 0, 7], [0, 4] + [0, 7] * 600])
+def test_groups_over_one_another(mk, torch_cuda, off):
+    """A group with tokens of an earlier one has none of its keys; the earlier one keeps its own, and every token its own
+    rows."""
+    torch = torch_cuda
+    H, KV, D = 4, 2, 64
+    b = Batch(np.random.default_rng(2), [(80, [(10, 2), (3, 2)]), (0, [(6, 1), (4, 2)])], KV, D, 1)
+    assert b.n == 8
+    q = queries(torch, BF16, b.n, H, D, 3)
+    base = b.prefix_base[0]
+    G = len(off) - 1
+    good = [off[g] < off[g + 1] and off[g] >= max([off[e + 1] for e in range(g) if off[e] < off[e + 1]] + [0])
+            for g in range(G)]
+    plain = b.keys_of
+    b.prefix_base, b.prefix_len = [base + g % 7 for g in range(G)], [80 - g % 11 - g % 7 for g in range(G)]
+    if G > 1000:
+        b.prefix_base, b.prefix_len = [base] * G, [80] + [30] * (G - 1)
+    b.group_off = off
+
+    def keys_of(i):
+        rows = []
+        for g in range(G):
+            if good[g] and off[g] <= i < off[g + 1]:
+                rows += list(range(b.prefix_base[g], b.prefix_base[g] + b.prefix_len[g]))
+        rows += list(range(b.kv_base[i], b.kv_base[i] + b.n_keys[i]))
+        return rows + [b.kv_base[i] + a for a in b.anc[i]]
+    b.keys_of = keys_of
+    got = call(mk, torch, BF16, b, q, H, KV, D, status=mk.MK_ERR_ARG)
+    check(torch, BF16, b, q, got, H, KV, D)
