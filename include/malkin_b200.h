@@ -367,8 +367,9 @@ int mk_qk_norm_rope(int type, const void* dev_qkv, int64_t ld, int n, int H, int
  * KV head h / (H / KV). dev_q and dev_out: n rows of H x D, dev_k and dev_v: n rows of KV x D, each with its own stride;
  * type MK_TYPE_F16 or MK_TYPE_BF16, D 64 or 128, buffers 16-byte aligned, strides multiples of 8, scale > 0.
  * Rows of no sequence are left as they were, and what masked rows hold (later tokens, other sequences, NaN or infinities
- * among them) does not reach an output. Offsets that descend or leave 0 .. n: that sequence's rows are left as they were
- * and MK_ERR_ARG is recorded. MK_ERR_TIMEOUT (recorded): a wait inside the kernel ran out, the outputs are not valid. */
+ * among them) does not reach an output. Offsets that descend or leave 0 .. n, or a sequence that begins before the end
+ * of an earlier one: it is left out, rows that only it has are left as they were, and MK_ERR_ARG is recorded.
+ * MK_ERR_TIMEOUT (recorded): a wait inside the kernel ran out, the outputs are not valid. */
 int mk_attention_prompt(int type, const void* dev_q, int64_t q_ld, const void* dev_k, int64_t k_ld, const void* dev_v,
                         int64_t v_ld, int n, int n_seq, const int32_t* dev_off, int H, int KV, int D, float scale,
                         void* dev_out, int64_t out_ld, int32_t* dev_status, void* stream);

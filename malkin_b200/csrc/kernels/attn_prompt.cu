@@ -73,20 +73,35 @@ constexpr int prompt_smem() {
 
 // The sequence and the 256-row tile that CTA `want` of a head takes: of each 32 sequences the tiles with the most keys first,
 // so that what runs last is short (eight prompts of up to 2048 tokens, 32 heads of 128: 225 us for 229 in sequence order). A
-// tile's place is found from the number of tiles at or above a depth, by bisection.
+// tile's place is found from the number of tiles at or above a depth, by bisection. A sequence that begins before the end of an
+// earlier one is left out, which takes a look at those ends from the first offset on that descends.
 __device__ __forceinline__ void find_tile(const int32_t* off, int n_seq, int n, int want, int lane, int* status,
                                           PromptSmall* sm) {
-  int lo_f = 0, hi_f = 0, tile_f = -1;
+  int lo_f = 0, hi_f = 0, tile_f = -1, until = 0;  // until: end of the sequences before the 32
+  bool falls = false;
   for (int s0 = 0; s0 < n_seq; s0 += 32) {
     const int s = s0 + lane;
     int lo = 0, hi = 0;
     if (s < n_seq) {
       lo = off[s];
       hi = off[s + 1];
-      if (lo < 0 || hi < lo || hi > n) {
-        if (status) atomicCAS(status, 0, kStatusBadIndex);
-        lo = hi = 0;
+    }
+    falls = __any_sync(0xffffffffu, hi < lo) || falls;
+    bool bad = lo < 0 || hi < lo || hi > n;
+    int end = !bad && hi > lo ? hi : 0;  // with the scan: of the sequences up to the lane's
+    if (falls) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end = max(end, y);
       }
+      const int before = max(until, __shfl_up_sync(0xffffffffu, end, 1) * (lane > 0));
+      bad |= hi > lo && lo < before;
+    }
+    until = max(until, __reduce_max_sync(0xffffffffu, end));
+    if (bad) {
+      if (status) atomicCAS(status, 0, kStatusBadIndex);
+      lo = hi = 0;
     }
     const int tiles = (hi - lo + kPair - 1) / kPair;
     const int all = warp_isum(tiles);
@@ -473,8 +488,9 @@ int run_prompt(const PromptArgs& a, bool bf16, cudaStream_t s) {
     if (at.numRegs * 3 < 2 * kPromptSoftmaxRegs + kPromptOtherRegs) return cudaErrorInvalidConfiguration;
     set[dev] = true;
   }
-  // a sequence of L rows has at most L / 256 + 1 tiles
-  const int64_t tiles = a.n / kPair + std::min<int64_t>(a.n_seq, a.n);
+  // a sequence of L rows has at most L / 256 + 1 tiles; one that is bad has none, so the last tile's search passes over all
+  // offsets then, and finds each that is
+  const int64_t tiles = a.n / kPair + std::min<int64_t>(a.n_seq, static_cast<int64_t>(a.n) + 1);
   const int64_t grid = tiles * a.H;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   k_attn_prompt<T, D><<<static_cast<unsigned>(grid), kPromptThreads, prompt_smem<D>(), s>>>(mq, mk, mv, a);

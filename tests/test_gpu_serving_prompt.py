@@ -227,3 +227,33 @@ def test_stream_and_graph(mk, torch_cuda):
     graph.replay()
     torch.cuda.synchronize()
     verify(0)
+
+
+@pytest.mark.parametrize("n,off,good", [
+    (1000, [0, 600, 0, 600, 0, 600, 1000], [0, 5]),  # the same rows three times: the first stands
+    (500, [0, 300, 100, 500], [0]),                  # the third begins inside the first
+    (500, [100, 300, 0, 400, 450], [0, 3]),          # or reaches over it
+    (4, [0, 1, 2, 3, 4] + [4] * 35 + [7], [0, 1, 2, 3]),  # a bad end behind more empty sequences than there are rows
+    (40, [0] * 70 + [40, 30], [69])])
+def test_offsets_that_are_bad_together(mk, torch_cuda, n, off, good):
+    """Every bad offset is recorded, also behind the last row; a sequence over an earlier one's rows is left out, and the
+    others are whole."""
+    torch = torch_cuda
+    H, KV, D = 4, 2, 64
+    wide = (H + 2 * KV) * D
+    buf = torch.randn(n, wide, generator=torch.Generator().manual_seed(n)).to(torch.bfloat16).cuda()
+    o = torch.tensor(off, dtype=torch.int32, device="cuda")
+    out = torch.full((n, H * D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    e = 2
+    mk.attention_prompt(BF16, buf.data_ptr(), wide, buf.data_ptr() + H * D * e, wide, buf.data_ptr() + (H + KV) * D * e,
+                        wide, n, len(off) - 1, o.data_ptr(), H, KV, D, D ** -0.5, out.data_ptr(), H * D + 8, st.data_ptr())
+    torch.cuda.synchronize()
+    assert int(st) == mk.MK_ERR_ARG
+    x, got = buf.float().cpu().numpy().astype(np.float64), out.float().cpu().numpy()
+    rest = np.ones(n, bool)
+    for s in good:
+        lo, hi = off[s], off[s + 1]
+        check(torch, BF16, x[lo:hi], [0, hi - lo], got[lo:hi], H, KV, D)
+        rest[lo:hi] = False
+    assert (got[rest] == 7).all()
