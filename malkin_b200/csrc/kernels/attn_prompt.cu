@@ -3,7 +3,8 @@
 // Row i of a sequence: out_i = sum_{j <= i} p_j v_j / sum p_j, p_j = exp(scale q_i k_j - m). One pass over the keys with
 // the running maximum and sum of the softmax per row (fp32), S = Q K^T and O += P V on tcgen05 with both accumulators in
 // TMEM. P is rounded to the operands' type (half a step of it, 2^-8 or 2^-11, of each weight; the sum of the weights is
-// taken before that rounding): tcgen05 has no wider A operand at this rate, and the errors of a row's weights average out.
+// taken before that rounding): tcgen05 has no wider A operand at this rate, and the errors of a row's weights average out. fp16
+// has no such steps below 2^-14, and its weights are kept 2^7 larger: those below 2^-21 of the largest are held to 2^-32 of it.
 //
 // A CTA takes 256 rows of one head as two tiles of 128, so each K / V tile read from L2 feeds two tiles, and one tile's
 // MMAs run while the other's softmax does:
@@ -12,8 +13,8 @@
 //   warp 8           issues every MMA      warp 9  TMA loads     warps 10, 11  check the V tiles of the diagonal
 // TMEM (512 columns): S0 | S1 | O0 | O1. Shared memory: both Q tiles and a ring of K and V tiles of 128 keys.
 //
-// The maximum used for a row is only raised when it grew by more than 8 in the exponent of 2 (weights stay below 2^8,
-// which both types hold), so that O is rarely rescaled.
+// The maximum used for a row is only raised when it grew by more than 8 in the exponent of 2 (weights stay below 2^8, in fp16
+// 2^15, which both types hold), so that O is rarely rescaled.
 //
 // Bound: the tensor pipe from some 300 tokens on (4 D H operations a pair of a row and a key). What holds it: per pair of
 // blocks of 128 keys 3670 cycles, of which the softmax takes 2200 and the four MMAs 1320, little of it at once, because both
@@ -50,6 +51,7 @@ constexpr int kKeys = 128;   // keys of a block
 constexpr int kPromptThreads = 384;
 constexpr int kPromptSoftmaxRegs = 208, kPromptOtherRegs = 88;  // 2 x 208 + 88 = 3 x the 168 of the launch
 constexpr float kRaise = 8.0f;
+constexpr float kHalfHeadroom = 7.0f;  // exponent of what fp16 weights are multiplied by; their sum carries it too
 
 template <int D>
 struct PromptShape {
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tmem_st32(to + 32 * b, v);
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : m * c;
+      const float mc = (m == -INFINITY ? 0.0f : m * c) - (std::is_same<T, __half>::value ? kHalfHeadroom : 0.0f);
       const f2 c2 = f2_make(c, c), m2 = f2_make(-mc, -mc);
       f2 sum2 = f2_make(0.0f, 0.0f), sum3 = sum2;
 #pragma unroll

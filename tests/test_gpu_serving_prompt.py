@@ -257,3 +257,26 @@ def test_offsets_that_are_bad_together(mk, torch_cuda, n, off, good):
         check(torch, BF16, x[lo:hi], [0, hi - lo], got[lo:hi], H, KV, D)
         rest[lo:hi] = False
     assert (got[rest] == 7).all()
+
+
+def test_many_small_weights(mk, torch_cuda):
+    """One key of weight 1 with a value of 0 and 1999 of weight 2^-25.4: together they are the output. fp16 holds weights
+    below its smallest normal number to 2^-32 of the largest (it keeps them 2^7 larger), so the row's sum is off by at most
+    half of that for each, on top of the rounding of the output."""
+    torch = torch_cuda
+    H = KV = 1
+    D, n, shift = 64, 2000, -17.609375
+
+    def one(buf, off):
+        buf[:] = 0
+        buf[:, 0] = 8.0           # the score of a key is its first value
+        buf[1:, D] = shift
+        buf[1:, 2 * D:] = 1.0
+
+    x, off, got, _ = run(mk, torch, F16, [n], H, KV, D, poison=one)
+    w = np.exp(shift)
+    i = np.arange(n)
+    want = i * w / (1 + i * w)
+    tol = i * 2.0 ** -32 + (2.0 ** -11 + 2.0 ** -12) * want + 2.0 ** -25
+    err = np.abs(got[:, :D] - want[:, None])
+    assert np.all(err <= tol[:, None]), (err.max(), want[-1], got[-1, 0])
