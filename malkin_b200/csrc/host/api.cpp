@@ -1,6 +1,7 @@
 // The C ABI (include/malkin_b200.h): status codes instead of exceptions, thread-local error text.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
@@ -143,12 +144,15 @@ void check_dev(std::initializer_list<DevArg> args, const char* who) {
 }
 
 int current_sms() {
-  static int sms[mkb::kMaxDevices] = {};  // the same for every caller: a race writes the same value
+  static std::atomic<int> sms[mkb::kMaxDevices] = {};
   const int dev = current_device();
   if (dev >= mkb::kMaxDevices) throw mkb::UnsupportedError("device ordinal out of range");
-  if (!sms[dev])
-    mkb::cuda_check(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev), "device attribute");
-  return sms[dev];
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    mkb::cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "device attribute");
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // Temporary quantized-activation buffers for the kernel-level entry points: int8 qx | the same int8 values in the

@@ -33,6 +33,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -475,7 +476,7 @@ int run_prompt(const PromptArgs& a, bool bf16, cudaStream_t s) {
   if (rc == 0) rc = make_map3(&mk, bf16, a.k, D, a.KV, a.n, a.k_ld, 64, kKeys);
   if (rc == 0) rc = make_map3(&mv, bf16, a.v, D, a.KV, a.n, a.v_ld, 64, kKeys);
   if (rc != 0) return rc;
-  static bool set[kMaxDevices] = {};
+  static std::atomic<bool> set[kMaxDevices] = {};  // several host threads may set the attributes at once
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;

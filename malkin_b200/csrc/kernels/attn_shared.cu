@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstddef>
 #include <type_traits>
@@ -1126,7 +1127,7 @@ __global__ void __launch_bounds__(256) k_shared_join(SharedArgs a, SharedWs w) {
 
 template <typename T, int D>
 int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
-  static bool set[kMaxDevices] = {};
+  static std::atomic<bool> set[kMaxDevices] = {};  // several host threads may set the attributes at once
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;

@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime_api.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace mkb {
@@ -14,7 +15,8 @@ inline int make_map3(CUtensorMap* map, bool bf16, const void* base, int width, i
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = nullptr;
+  static std::atomic<Encode> known{nullptr};  // calls from several host threads may look it up at once
+  Encode encode = known.load(std::memory_order_acquire);
   if (!encode) {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -22,6 +24,7 @@ inline int make_map3(CUtensorMap* map, bool bf16, const void* base, int width, i
     if (e != cudaSuccess) return e;
     if (found != cudaDriverEntryPointSuccess || !f) return cudaErrorNotSupported;
     encode = reinterpret_cast<Encode>(f);
+    known.store(encode, std::memory_order_release);
   }
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads),
                               static_cast<cuuint64_t>(rows)};

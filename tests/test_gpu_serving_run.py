@@ -240,3 +240,34 @@ def test_offsets_beyond_32_bits(mk, torch_cuda):
     want = ref.verify(lg.float().cpu().numpy().astype(np.float64), [0, 597, 600], draft.cpu().numpy(), None,
                       [1.0, 1.0], u.cpu().numpy())
     check_verify((n_acc.cpu().numpy(), nxt.cpu().numpy(), p.cpu().numpy(), int(st)), want, 598)
+
+
+def test_steps_from_several_host_threads(mk, torch_cuda):
+    """Four host threads at once, each with a step and a stream of its own: the results are those of the calls made alone."""
+    import threading
+    torch = torch_cuda
+    steps = [Step(torch, mk, (F16, BF16)[i % 2], 30 + i) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in steps]
+    for s in steps:
+        s.fill()
+        s.run(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = [s.results() for s in steps]
+    failed = []
+
+    def work(s, q):
+        try:
+            with torch.cuda.stream(q):
+                for _ in range(20):
+                    s.run(q.cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in zip(steps, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for s, w in zip(steps, want):
+        assert all(torch.equal(a, b) for a, b in zip(s.results(), w))
