@@ -1157,11 +1157,11 @@ int run_shared(const SharedArgs& a, void* ws, int sms, cudaStream_t s) {
   k_shared_plan<<<1, kPlanThreads, 0, s>>>(a, w, ctas);
   e = cudaGetLastError();
   if (e == cudaSuccess)
-    e = launch_pdl(k_shared_attend<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(kAttendThreads), shared_smem<D>(), s, 1,
+    e = launch_pdl(k_shared_attend<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(kAttendThreads), shared_smem<D>(), s,
                    mq, a, w);
   const int64_t warps = static_cast<int64_t>(a.n) * a.H;
   if (e == cudaSuccess)
-    e = launch_pdl(k_shared_join<T, D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, s, 1, a, w);
+    e = launch_pdl(k_shared_join<T, D>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, s, a, w);
   return e;
 }
 

@@ -10,25 +10,18 @@ __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.laun
 // Everything the kernel before this one wrote can be read (a plain launch: returns at once).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// cluster: CTAs of a cluster (1: none).
 template <typename... P, typename... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, A... args) {
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (cluster > 1) {
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
-  }
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 

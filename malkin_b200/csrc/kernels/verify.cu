@@ -596,13 +596,13 @@ int run_verify(const VerifyArgs& a, int sms, cudaStream_t s) {
   const int most = std::max(1, 4 * sms / a.n_req), per = static_cast<int>((y.chunks + most - 1) / most);
   const dim3 walk(static_cast<unsigned>((y.chunks + per - 1) / per), static_cast<unsigned>(a.n_req));
   if (e == cudaSuccess)
-    e = launch_pdl(k_verify_norm<T>, walk, dim3(kDrawThreads), 0, s, 1, a, n_chunks, static_cast<const RowPart*>(parts),
+    e = launch_pdl(k_verify_norm<T>, walk, dim3(kDrawThreads), 0, s, a, n_chunks, static_cast<const RowPart*>(parts),
                    decide, zpart, static_cast<int>(y.chunks), per);
   if (e == cudaSuccess)
-    e = launch_pdl(k_verify_rest<T>, grid, dim3(kDrawThreads), 0, s, 1, a, static_cast<const Decision*>(decide),
+    e = launch_pdl(k_verify_rest<T>, grid, dim3(kDrawThreads), 0, s, a, static_cast<const Decision*>(decide),
                    static_cast<const double*>(zpart), rpart, zsum);
   if (e == cudaSuccess)
-    e = launch_pdl(k_verify_pick<T>, dim3(static_cast<unsigned>(a.n_req)), dim3(kPickThreads), 0, s, 1, a,
+    e = launch_pdl(k_verify_pick<T>, dim3(static_cast<unsigned>(a.n_req)), dim3(kPickThreads), 0, s, a,
                    static_cast<const Decision*>(decide), static_cast<const double*>(zpart),
                    static_cast<const double*>(rpart), static_cast<const double*>(zsum), static_cast<int>(y.chunks));
   return e;
