@@ -2,7 +2,7 @@
 //
 // A token's keys are the prefix rows of its group, the first n_keys rows of its own sequence, and its ancestors' rows in
 // a draft tree. The prefix part is computed once per group for the rows (tokens x query heads of one KV head) of all its
-// requests, so its K and V are read once for up to 128 rows; the own part once per run of tokens with the same sequence.
+// requests, so its K and V are read once for up to 256 rows; the own part once per run of tokens with the same sequence.
 // Softmax parts are joined from (maximum, sum, unnormalised output) triples in fp32.
 //
 //   k_shared_plan     one CTA: tiles of up to 256 rows over (group, prefix) and (run, own rows); the blocks of 96 keys of

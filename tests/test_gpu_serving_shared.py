@@ -399,3 +399,32 @@ def test_groups_over_one_another(mk, torch_cuda, off):
     b.keys_of = keys_of
     got = call(mk, torch, BF16, b, q, H, KV, D, status=mk.MK_ERR_ARG)
     check(torch, BF16, b, q, got, H, KV, D)
+
+
+@pytest.mark.parametrize("H,KV", [(8, 2), (6, 2)])  # 32 and 42 tokens a stream (126 of its 128 rows)
+@pytest.mark.parametrize("keys", [95, 96, 97, 191, 192, 193])
+def test_around_blocks_and_tiles(mk, torch_cuda, H, KV, keys):
+    """Prefixes and own rows that end at a block of 96 keys, one before and one behind it; groups and runs of as many tokens
+    as a stream or a tile of two streams takes, one fewer and one more."""
+    torch = torch_cuda
+    D, half = 64, 128 // (H // KV)
+    groups = [(keys, [(keys - 1, 1), (keys, 2)])]
+    groups += [(keys if toks % 2 else 0, [(keys - 2, toks)]) for toks in (half - 1, half, half + 1)]
+    groups += [(keys, [(3, 1)] * toks) for toks in (2 * half - 1, 2 * half, 2 * half + 1)]
+    b = Batch(np.random.default_rng(keys), groups, KV, D, 1)
+    for t in (F16, BF16):
+        q = queries(torch, t, b.n, H, D, keys)
+        check(torch, t, b, q, call(mk, torch, t, b, q, H, KV, D), H, KV, D)
+
+
+@pytest.mark.parametrize("cached", [1, 300])
+def test_prompt_rows_behind_cached_ones(mk, torch_cuda, cached):
+    """The rest of a prompt whose first rows are in the cache: a run of tokens over one sequence whose n_keys rise by one,
+    more of them than a tile takes."""
+    torch = torch_cuda
+    H, KV, D = 8, 2, 128
+    b = Batch(np.random.default_rng(cached), [(0, [(cached, 200)]), (64, [(cached + 1, 70)])], KV, D)
+    for i in range(b.n):
+        b.n_keys[i] += 1  # each token sees its own row, which is in the cache before the call
+    q = queries(torch, BF16, b.n, H, D, 1)
+    check(torch, BF16, b, q, call(mk, torch, BF16, b, q, H, KV, D), H, KV, D)
