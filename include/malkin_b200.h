@@ -415,7 +415,7 @@ int mk_attention_shared(int type, const void* dev_q, int64_t q_ld, int n, int H,
  * lowest index of the maximum), next = argmax; dev_q and the uniforms are not used.
  * Results: dev_n_acc[r] drafts kept, dev_next[r], dev_p[x - r] (NULL: not wanted) the target's probability of each draft
  * looked at, 0 for those after the first one that was not kept. It comes from a row sum of 32-bit exponentials: within
- * 2^-16 of itself, 2^-23 as a rule. What is decided (kept or not, the token drawn) follows 64-bit sums to some 10^-13. A
+ * 2^-16 of itself, 2^-21 as a rule. What is decided (kept or not, the token drawn) follows 64-bit sums to some 10^-13. A
  * draft outside 0 .. V - 1 has probability 0. Logits of -infinity are tokens that cannot be drawn, NaN logits count as
  * -infinity; a row whose maximum is not finite has no distribution: no draft is kept on it, and as the row drawn from it
  * gives dev_next = -1. A request whose rows are not as above, or that has rows or drafts of an earlier one whose rows are

@@ -16,12 +16,15 @@
 // The maximum used for a row is only raised when it grew by more than 8 in the exponent of 2 (weights stay below 2^8, in fp16
 // 2^15, which both types hold), so that O is rarely rescaled.
 //
-// Bound: the tensor pipe from some 300 tokens on (4 D H operations a pair of a row and a key). What holds it: per pair of
-// blocks of 128 keys 3670 cycles, of which the softmax takes 2200 and the four MMAs 1320, little of it at once, because both
-// tiles' S and O fill TMEM and no scores can be computed ahead. Measured: 8192 tokens, 40 / 8 heads of 128, fp16: 614 to
-// 622 us (1.1 PFLOP/s) in bursts, 710 in a loop of seconds, under the power limit; eight prompts of up to 2048 tokens, 32 / 8
-// heads, bf16: 209 to 220 us. Not kept, at the long prompt: two threads a row 692 us; 64-key blocks with S in two buffers 777;
-// 2^x by a polynomial on the FMA pipe for 1/4 of the weights 626 against 632 in the same run, for 3/8 664.
+// Bound: the tensor pipe from some 300 tokens on (4 D H operations a pair of a row and a key). What holds it: a pair of blocks
+// of 128 keys (one for each tile) takes 3670 cycles at D 128; the tensor pipe works 2050 of them (four products of 512 each), a
+// tile's softmax takes 2200. A tile's softmax, its P V and its next Q K follow one another, and with two tiles in turn both the
+// tensor and the XU pipe idle for almost half of the time. TMEM has room to break that chain, which is not done: P leaves half
+// of its S's columns free, and at D 64 128 columns are not used at all. Measured: 8192 tokens, 40 / 8 heads of 128, fp16: 628 us
+// (1.1 PFLOP/s) in bursts, 716 to 720 in a loop of seconds, under the power limit (with weights not kept larger 621 and 712);
+// eight prompts of up to 2048 tokens, 32 / 8 heads, bf16: 211 to 220 us. Not kept, at the long prompt: two threads a row 692 us;
+// 64-key blocks with S in two buffers 777; 2^x by a polynomial on the FMA pipe for 1/4 of the weights 626 against 632 in the
+// same run, for 3/8 664.
 //
 // Masked keys: scores above the diagonal are replaced by -inf, whatever K holds there. Their weight 0 would still make a
 // NaN of an infinity or NaN in V, so the tiles on the diagonal, whose keys some rows must not see (later tokens, or the

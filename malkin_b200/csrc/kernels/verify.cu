@@ -15,11 +15,13 @@
 //   k_verify_pick  one CTA per request: the chunk, the segment and the token the running sum reaches its target in
 // A running sum over 151936 entries that is compared with a border has to be the same for whoever forms it, so the drawn
 // row's exponentials and sums are in 64 bits: with 32 the drawn index would differ from the exact one about once in 10^4
-// draws. An acceptance compares with one probability: its exponential is in 64 bits, its row's sum is k_verify_rows' of 32-bit
-// exponentials (off by 8e-8 of itself as a rule), and where that could decide, the row is summed again in 64 bits. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared memory were
-// slower: 93, 85 and 96 us against 75 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM three times.)
-// Measured, V = 151936: 64 requests of 5 fp32 rows with probabilities 75 to 78 us, of which k_verify_rows 35 (5.6 TB/s, 0.85 of
-// a copy's rate); one request of 9 fp32 rows 19 us, 8 requests of up to 9 bf16 rows 24, both held by four dependent launches.
+// draws. An acceptance compares with one probability: its exponential is in 64 bits, its row's sum is k_verify_rows' of
+// 32-bit exponentials (4e-7 of itself at most over the measured rows), and where that could decide, the row is summed again
+// in 64 bits. All sums are taken in a fixed order. (Clusters of 4, 8 or 16 CTAs a request that kept the row in shared
+// memory were slower: 93, 85 and 96 us against 75 us at 64 requests of 5 rows; a cluster barrier waits for its slowest SM
+// three times.)
+// Measured, V = 151936: 64 requests of 5 fp32 rows with probabilities 79 us, of which k_verify_rows 35 (5.6 TB/s, 0.85 of a
+// copy's rate); one request of 9 fp32 rows 19 us, 8 requests of up to 9 bf16 rows 24, both held by four dependent launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
