@@ -21,11 +21,11 @@
 // most 4 of those 20 bits and spares the sums (two prefixes of 32768 rows: 257 us, with the sums in every block 263; the block's
 // largest scale alone, seen by the row or not, 246, and wrong where scales lie far apart).
 // Bound: HBM for one tile of rows a group (128 rows: 65.5 kFLOP against 264 bytes a key and head, the machine's balance),
-// the tensor pipe and the conversion above that. What holds it: a block of 96 keys took 3700 cycles for 128 rows and 3900 for
-// 256 (now some 4 % more), 2500 of them the widening (K to bf16 1700, V to fp16 800); the plan takes 7 us, finding a piece's place 2, the join 4 to
-// 5. Measured, with queries of 32 / 8 heads of 128: two prefixes of up to 32768 rows with 32 requests of 4 rows each, bf16:
-// 257 us; 8 trees of 17 rows behind 2048 rows, fp16: 44; 4 single rows behind 1000, 16 / 8 heads, bf16: 25. Two CTAs an
-// SM with blocks of 64 keys took 497 us at the first.
+// the tensor pipe and the conversion above that. What holds it: a block of 96 keys took 3700 cycles for 128 rows and 3900
+// for 256 (now some 4 % more), 2500 of them the widening (K to bf16 1700, V to fp16 800); the plan takes 7 us, finding a
+// piece's place 2, the join 4 to 5. Measured, with queries of 32 / 8 heads of 128: two prefixes of up to 32768 rows with 32
+// requests of 4 rows each, bf16: 257 us; 8 trees of 17 rows behind 2048 rows, fp16: 45; 4 single rows behind 1000, 16 / 8
+// heads, bf16: 27. Two CTAs an SM with blocks of 64 keys took 497 us at the first.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
